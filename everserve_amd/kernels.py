@@ -250,6 +250,19 @@ _SIGNATURES: tuple[tuple[str, object, tuple], ...] = (
     ("evs_ipc_open", _I32, (_P, _I64, _P)),
     ("evs_ipc_close", _I32, (_P,)),
     ("evs_wall_clock_khz", _I32, (_P,)),
+    ("evs_fp4_row_bytes", _I32, (_I64, _P)),
+    ("evs_fp4_write_rows", _I32,
+     (_P, _P, _P, _I32, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P)),
+    ("evs_fp4_read_rows", _I32, (_P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I32, _P)),
+    ("evs_fp4_attend_workspace", _I32, (_I64, _I64, _I64, _I64, _I64, _I64, _I64, _P)),
+    ("evs_fp4_attend", _I32,
+     (_P, _P, _I32, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P,
+      _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P)),
+    ("evs_copy_blocks", _I32,
+     (_P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _P)),
+    ("evs_plan_compaction_workspace", _I32, (_I64, _P)),
+    ("evs_plan_compaction", _I32,
+     (_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P)),
 )
 ENTRY_POINTS = tuple(name for name, _, _ in _SIGNATURES)
 
@@ -270,11 +283,21 @@ def open_library(path: Path | None = None) -> ctypes.CDLL:
     return lib
 
 
+@functools.lru_cache(maxsize=1)
+def _row_types() -> dict:
+    """The library's number of each element type of full-width rows (EVS_BF16, EVS_F16, EVS_F32)."""
+    import torch
+
+    return {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
 # A small call costs the host more than the GPU, and these helpers were most of it: through
 # torch.cuda.current_stream, torch.cuda.device and sets of torch.device objects a gather of 8 slots
 # took 8.4 us of host time and order_pairs 13.2, through the raw stream and the devices' numbers
 # 6.2 and 6.3, of which HIP's launch is 3.2.
 _FIVE = ctypes.c_int64 * 5
+_FOUR = ctypes.c_int64 * 4
+_TWO = ctypes.c_int64 * 2
 _HERE = contextlib.nullcontext()
 
 
@@ -710,6 +733,205 @@ class Kernels:
                                        int(bounce_bytes), int(max_threads),
                                        int(stream.cuda_stream))
         )
+
+    # -------------------------------------------------------------- a cache held in 4 bits
+    def fp4_write_rows(self, key, value, slots, cache, num_blocks: int, block_size: int,
+                       strides: Sequence[int]) -> None:
+        """Round the rows ``key`` and ``value`` ([n, heads, d], bf16, f16 or f32, any strides but
+        the last's) to 4 bits and write them at ``slots`` (int64 [n]) of the 4-bit ``cache``, a
+        uint8 device tensor addressed by five byte strides. A slot outside the cache is padding
+        and is skipped; slots must be distinct."""
+        import torch
+
+        types = _row_types()
+        if key.dim() != 3 or key.shape != value.shape or slots.numel() != key.shape[0]:
+            raise RuntimeError(f"fp4_write_rows: {slots.numel()} slots, keys of shape "
+                               f"{tuple(key.shape)} and values of {tuple(value.shape)}")
+        if key.dtype != value.dtype or key.dtype not in types:
+            raise RuntimeError(f"fp4_write_rows: rows of {key.dtype} and {value.dtype}: both must "
+                               "be bf16, f16 or f32")
+        if not (key.is_cuda and value.is_cuda and cache.is_cuda):
+            raise RuntimeError("fp4_write_rows: the rows and the cache must be on the device")
+        n, heads, d = key.shape
+        ks, vs = key.stride(), value.stride()
+        if ks[2] != 1 or vs[2] != 1:
+            raise RuntimeError("fp4_write_rows: a row's elements must be contiguous")
+        sp = _device_ptr(slots, "fp4_write_rows: slots", torch.long)
+        _one_device("fp4_write_rows", key, value, slots, cache)
+        with _on_device_of(cache):
+            self._check(
+                self._lib.evs_fp4_write_rows(
+                    key.data_ptr(), value.data_ptr(), _FOUR(ks[0], ks[1], vs[0], vs[1]),
+                    types[key.dtype], sp, n, cache.data_ptr(), num_blocks, block_size, heads, d,
+                    _FIVE(*strides), _stream_of(cache.device),
+                )
+            )
+
+    def fp4_read_rows(self, cache, num_blocks: int, block_size: int, heads: int, d: int,
+                      strides: Sequence[int], slots, dtype):
+        """The rows at ``slots`` (int64 [n]) of a 4-bit ``cache`` at full width: new tensors
+        ``key`` and ``value`` ``[n, heads, d]`` of ``dtype`` (bf16, f16 or f32). A slot outside
+        the cache reads as zeros."""
+        import torch
+
+        types = _row_types()
+        if dtype not in types:
+            raise RuntimeError(f"fp4_read_rows: rows of {dtype}: bf16, f16 or f32")
+        if not cache.is_cuda:
+            raise RuntimeError("fp4_read_rows: the cache must be on the device")
+        sp = _device_ptr(slots, "fp4_read_rows: slots", torch.long)
+        _one_device("fp4_read_rows", cache, slots)
+        n = slots.numel()
+        key = torch.empty((n, heads, d), dtype=dtype, device=cache.device)
+        value = torch.empty((n, heads, d), dtype=dtype, device=cache.device)
+        with _on_device_of(cache):
+            self._check(
+                self._lib.evs_fp4_read_rows(
+                    cache.data_ptr(), num_blocks, block_size, heads, d, _FIVE(*strides), sp, n,
+                    key.data_ptr(), value.data_ptr(), types[dtype], _stream_of(cache.device),
+                )
+            )
+        return key, value
+
+    def fp4_attend(self, q, cache, num_blocks: int, block_size: int, heads: int,
+                   strides: Sequence[int], block_tables, seq_lens, q_starts=None,
+                   max_q: int | None = None, scale: float | None = None, max_len: int = 0,
+                   out=None, return_lse: bool = False):
+        """Attention of ``q`` ([tokens, q_heads, d], bf16 or f16) over a 4-bit ``cache``.
+
+        Sequence s has ``seq_lens[s]`` tokens in the pages ``block_tables[s]`` (int32) and the
+        queries ``q_starts[s]`` to ``q_starts[s + 1]`` (int32 [seqs + 1]; None: query s alone),
+        its last tokens, each of which sees the tokens up to itself. ``max_q`` is at least the
+        most queries of a sequence (None: one without ``q_starts``, else all of them), ``scale``
+        defaults to d ** -0.5, ``max_len`` is at least the longest length if given. Returns
+        ``out`` ([tokens, q_heads, d], written into if given), with ``return_lse`` also the f32
+        [tokens, q_heads] logs of the sums of exp(scores). A row that sees nothing is zeros, its
+        log -infinity; a page id outside the cache holds nothing. There is no backward pass.
+        Enqueued on the current stream; its workspace comes from torch's allocator."""
+        import torch
+
+        type_ = _row_types().get(q.dtype, 2)
+        if q.dim() != 3 or type_ == 2 or not q.is_cuda:
+            raise RuntimeError(f"fp4_attend: queries are [tokens, heads, d] in bf16 or f16 on the "
+                               f"device, not {q.dtype} of shape {tuple(q.shape)}")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("fp4_attend: no backward pass: detach the queries")
+        tokens, q_heads, d = q.shape
+        qs = q.stride()
+        if qs[2] != 1:
+            raise RuntimeError("fp4_attend: a query's elements must be contiguous")
+        if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or (
+                block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+            raise RuntimeError("fp4_attend: block_tables are int32 [seqs, pages], a row contiguous")
+        seqs, width = block_tables.shape
+        lp = _device_ptr(seq_lens, "fp4_attend: seq_lens", torch.int32)
+        if seq_lens.numel() != seqs:
+            raise RuntimeError(f"fp4_attend: {seqs} block tables but {seq_lens.numel()} lengths")
+        starts = 0
+        if q_starts is not None:
+            starts = _device_ptr(q_starts, "fp4_attend: q_starts", torch.int32)
+            if q_starts.numel() != seqs + 1:
+                raise RuntimeError(f"fp4_attend: {seqs} sequences need {seqs + 1} query starts, "
+                                   f"got {q_starts.numel()}")
+        if max_q is None:
+            max_q = 1 if q_starts is None else tokens
+        if not (cache.is_cuda and block_tables.is_cuda):
+            raise RuntimeError("fp4_attend: the cache and the tables must be on the device")
+        if out is None:
+            out = torch.empty((tokens, q_heads, d), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise RuntimeError("fp4_attend: out must be contiguous and like the queries")
+        lse = None
+        if return_lse:
+            lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
+        _one_device("fp4_attend", q, cache, block_tables, seq_lens, q_starts, out)
+        need = ctypes.c_int64()
+        with _on_device_of(q):
+            self._check(self._lib.evs_fp4_attend_workspace(
+                seqs, tokens, q_heads, heads, d, max_q, max_len or width * block_size,
+                ctypes.byref(need)))
+            work = None
+            if need.value:
+                work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            self._check(
+                self._lib.evs_fp4_attend(
+                    q.data_ptr(), _TWO(qs[0], qs[1]), type_, out.data_ptr(),
+                    lse.data_ptr() if return_lse else None, tokens, q_heads, cache.data_ptr(),
+                    num_blocks, block_size, heads, d, _FIVE(*strides), block_tables.data_ptr(),
+                    block_tables.stride(0), width, lp, starts or None, seqs, max_q,
+                    max_len or width * block_size, d ** -0.5 if scale is None else scale,
+                    work.data_ptr() if need.value else None, need.value, _stream_of(q.device),
+                )
+            )
+        return (out, lse) if return_lse else out
+
+    # -------------------------------------------------------------- pages of a cache
+    def copy_blocks(self, layer_ptrs, src, dst, num_blocks: int, heads: int, d: int,
+                    block_size: int, strides: Sequence[int], elem_size: int, count=None) -> None:
+        """Copy page ``src[i]`` to page ``dst[i]`` (int32) of every layer's cache, whole.
+
+        ``count`` (int32 [1], on the device) cuts the list short. A pair with an id outside the
+        cache moves nothing. Destinations must be distinct, and none a pair's source."""
+        import torch
+
+        if len(strides) != 5:
+            raise RuntimeError("copy_blocks: a layout is five strides")
+        if src.numel() != dst.numel():
+            raise RuntimeError(f"copy_blocks: {src.numel()} sources but {dst.numel()} destinations")
+        lp = _device_ptr(layer_ptrs, "copy_blocks: layer_ptrs", torch.long)
+        sp = _device_ptr(src, "copy_blocks: src", torch.int32)
+        dp = _device_ptr(dst, "copy_blocks: dst", torch.int32)
+        cp = None if count is None else _device_ptr(count, "copy_blocks: count", torch.int32)
+        if count is not None and count.numel() != 1:
+            raise RuntimeError(f"copy_blocks: one count, not {count.numel()}")
+        _one_device("copy_blocks", layer_ptrs, src, dst, count)
+        with _on_device_of(src):
+            self._check(
+                self._lib.evs_copy_blocks(
+                    lp, layer_ptrs.numel(), sp, dp, src.numel(), cp, int(num_blocks), int(heads),
+                    int(d), int(block_size), _FIVE(*strides), int(elem_size),
+                    _stream_of(src.device),
+                )
+            )
+
+    def plan_compaction(self, block_tables, counts, num_blocks: int):
+        """The moves that pack the pages that ``block_tables`` (int32 [rows, width], of row r the
+        first ``counts[r]`` entries, int32; None: all) name to the front of a cache of
+        ``num_blocks`` pages: new tensors ``(tables, src, dst, sizes)``, ``sizes`` = [pages in use,
+        moves]; ``src`` and ``dst`` ([num_blocks // 2]) hold -1 past the moves. Nothing is
+        synchronised: :meth:`copy_blocks` takes ``sizes[1:]`` as its count."""
+        import torch
+
+        if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or (
+                not block_tables.is_cuda) or (
+                block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+            raise RuntimeError("plan_compaction: block_tables are int32 [rows, pages] on the "
+                               "device, a row contiguous")
+        rows, width = block_tables.shape
+        cp = None
+        if counts is not None:
+            cp = _device_ptr(counts, "plan_compaction: counts", torch.int32)
+            if counts.numel() != rows:
+                raise RuntimeError(f"plan_compaction: {rows} rows but {counts.numel()} counts")
+        _one_device("plan_compaction", block_tables, counts)
+        num_blocks = int(num_blocks)
+        room = max(0, num_blocks // 2)
+        dev = block_tables.device
+        tables = torch.empty((rows, width), dtype=torch.int32, device=dev)
+        need = ctypes.c_int64()
+        self._check(self._lib.evs_plan_compaction_workspace(num_blocks, ctypes.byref(need)))
+        ints = torch.empty(2 * room + 2, dtype=torch.int32, device=dev)
+        src, dst, sizes = ints[:room], ints[room:2 * room], ints[2 * room:]
+        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        with _on_device_of(block_tables):
+            self._check(
+                self._lib.evs_plan_compaction(
+                    block_tables.data_ptr(), rows, width, block_tables.stride(0), cp, num_blocks,
+                    tables.data_ptr(), src.data_ptr(), dst.data_ptr(), room, sizes.data_ptr(),
+                    work.data_ptr(), need.value, _stream_of(dev),
+                )
+            )
+        return tables, src, dst, sizes
 
     # -------------------------------------------------------------- the store's commit copy
     def store_commit_plan(self, stage_offsets, tables, written_step, crc, num_slots: int,

@@ -213,6 +213,92 @@ int evs_slot_all_reduce(const void* inp, void* out, int64_t n, const int64_t* bu
  * (core/csrc/slot.cu:229-232). Writes the count to *out. */
 int evs_slot_blocks(int64_t maxn, int64_t words, int64_t* out);
 
+/* ---- A paged cache held in 4 bits, and the pages of any cache. None of these has a counterpart in
+ * the reference, whose caches are its engine's. ----
+ *
+ * A 4-bit half-row is the K or the V of one slot and head, head_dim elements (a multiple of 8, 16 to
+ * 256): head_dim / 2 bytes of E2M1 codes (element j in bits 4 (j % 8) of dword j / 8), one scale
+ * byte for each 32 elements (the codes' factor 2^(byte - 127); 255: the group holds no number and
+ * reads as NaN), zeros up to a multiple of 4 bytes: evs_fp4_row_bytes in all. A 4-bit cache is
+ * such half-rows in any of the cache layouts: to the gathers, scatters, the stager and the restore it
+ * is a cache of 1-byte elements whose head size is the half-row's bytes. `strides` (host array of
+ * five, in bytes: page, slot in page, head, K to V, 1) and the cache's address are multiples of 4.
+ * Element types of full-width rows: */
+#define EVS_BF16 0
+#define EVS_F16 1
+#define EVS_F32 2
+int evs_fp4_row_bytes(int64_t head_dim, int64_t* bytes);
+
+/* Round the K and V rows of n slots to 4 bits and write them: row i of `key` and `value` ([n, heads,
+ * head_dim] elements of `type`, contiguous in the last; in_strides: key's token and head strides,
+ * then value's, in elements) goes to slot slots[i] (device, int64) of every head. A slot outside
+ * [0, num_blocks * block_size) is padding and is skipped. Slots must be distinct, as for
+ * evs_scatter_rows. A group's scale is the least power of two, from 2^-126 to 2^125, that brings
+ * its largest magnitude to 7 or below; codes are the nearest, ties to even, up to 6. A group with
+ * an infinity or a NaN gets scale byte 255. */
+int evs_fp4_write_rows(const void* key, const void* value, const int64_t* in_strides, int type,
+                       const int64_t* slots, int64_t n, void* cache, int64_t num_blocks,
+                       int64_t block_size, int64_t heads, int64_t head_dim,
+                       const int64_t* strides, void* stream);
+
+/* The rows of n slots at full width: contiguous key and value [n, heads, head_dim] of `type`, each
+ * starting on 16 bytes. A slot outside the cache reads as zeros. Exact for bf16 and f32. */
+int evs_fp4_read_rows(const void* cache, int64_t num_blocks, int64_t block_size, int64_t heads,
+                      int64_t head_dim, const int64_t* strides, const int64_t* slots, int64_t n,
+                      void* key, void* value, int type, void* stream);
+
+/* Attention of query rows over a 4-bit cache. Sequence s has the context of its first lens[s] tokens
+ * (device, int32), token t at slot t % block_size of page tables[s][t / block_size] (device, int32,
+ * rows of `width` entries, table_stride apart), and the queries q_starts[s] .. q_starts[s + 1] - 1
+ * (device, int32 [seqs + 1], ascending; NULL: query s alone, tokens == seqs), which are its last
+ * tokens: query i of nq is at position lens[s] - nq + i and sees the tokens up to its own. Query
+ * head h reads KV head h / (q_heads / heads).
+ *   q     [tokens, q_heads, head_dim] of `type` (EVS_BF16 or EVS_F16), contiguous in the last;
+ *         q_strides: token and head strides in elements;
+ *   out   contiguous [tokens, q_heads, head_dim] of `type`, starting on 16 bytes;
+ *   lse   contiguous f32 [tokens, q_heads], the natural log of the sum of exp(scores), or NULL.
+ * A row that sees nothing gives zeros, and lse -infinity. A table entry outside [0, num_blocks)
+ * holds nothing: its tokens are masked. A length is taken up to width * block_size, a sequence's
+ * queries up to max_q and `tokens`. Queries that no sequence names are not written. `max_len` (0:
+ * width * block_size) is at least the longest length, and only steers how the work is split.
+ * `workspace` is device memory of evs_fp4_attend_workspace bytes for the same counts, 16-byte
+ * aligned, that no overlapping call uses. The call allocates nothing and may be captured. */
+int evs_fp4_attend_workspace(int64_t seqs, int64_t tokens, int64_t q_heads, int64_t heads,
+                             int64_t head_dim, int64_t max_q, int64_t max_len, int64_t* bytes);
+int evs_fp4_attend(const void* q, const int64_t* q_strides, int type, void* out, float* lse,
+                   int64_t tokens, int64_t q_heads, const void* cache, int64_t num_blocks,
+                   int64_t block_size, int64_t heads, int64_t head_dim, const int64_t* strides,
+                   const int32_t* tables, int64_t table_stride, int64_t width,
+                   const int32_t* lens, const int32_t* q_starts, int64_t seqs, int64_t max_q,
+                   int64_t max_len, float scale, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/* Copy page src[i] to page dst[i] (device, int32), every slot, head, K and V, in every layer:
+ * caches addressed as in evs_gather_rows (strides in elements, all positive), num_blocks pages
+ * each. `count` (device, int32), if not NULL, cuts the list short. A pair with an id outside
+ * [0, num_blocks), or src == dst, moves nothing. Destinations must be distinct and none may be
+ * another pair's source. Where every stride and run of a page is a multiple of 16 bytes the layer
+ * bases must be too, as for evs_gather_rows. */
+int evs_copy_blocks(const int64_t* layer_ptrs, int64_t num_layers, const int32_t* src,
+                    const int32_t* dst, int64_t num_pairs, const int32_t* count,
+                    int64_t num_blocks, int64_t num_heads, int64_t head_dim, int64_t block_size,
+                    const int64_t* strides, int64_t elem_size, void* stream);
+
+/* Plan the moves that pack a cache's used pages to its front. The used pages are those that the
+ * block tables name (device, int32 [rows, width], rows row_stride apart; of row r the first
+ * counts[r] entries, device, int32, NULL: all), each once however often it is named; entries
+ * outside [0, num_blocks) are ignored. With u of them, the ones at ids of u and above move, in
+ * order, to the unused ids below u, in order: src[i] to dst[i], i < sizes[1], and -1 from there to
+ * `room` (at least num_blocks / 2). tables_out (contiguous [rows, width]) are the tables with the
+ * new ids, entries not in use as they were; sizes = [u, moves]. evs_copy_blocks with
+ * count = sizes + 1 then moves the pages (a source is never a destination), and pages u and above
+ * are free. `workspace` is device memory of evs_plan_compaction_workspace bytes, 4-byte aligned. */
+int evs_plan_compaction_workspace(int64_t num_blocks, int64_t* bytes);
+int evs_plan_compaction(const int32_t* tables, int64_t rows, int64_t width, int64_t row_stride,
+                        const int32_t* counts, int64_t num_blocks, int32_t* tables_out,
+                        int32_t* src, int32_t* dst, int64_t room, int32_t* sizes,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Pin `bytes` of host memory at `ptr`, mapped into the device address space; *device_ptr receives
  * the address kernels use. Replaces host_register_mapped (core/csrc/gather.cu:137-144). */
 int evs_host_register_mapped(void* ptr, int64_t bytes, void** device_ptr);
