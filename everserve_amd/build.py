@@ -29,8 +29,9 @@ INCLUDE = ROOT / "include"
 LIBRARY = "libeverserve_mi355x.so"
 STAMP = "stamp.json"
 SOURCES = ("rows.hip", "order.hip", "reduce.hip", "slot.hip", "host_rows.hip", "store.hip",
-           "runtime.hip", "fp4.hip", "attend.hip", "pages.hip")
-HEADERS = ("common.hpp", "fp4.hpp", "host_copy.hpp", "workers.hpp")
+           "runtime.hip", "fp4.hip", "attend.hip", "attend_few.hip", "attend_many.hip",
+           "pages.hip")
+HEADERS = ("attend.hpp", "common.hpp", "fp4.hpp", "host_copy.hpp", "workers.hpp")
 PUBLIC_HEADERS = ("everserve_mi355x.h",)
 DEFAULT_ARCHS = "gfx950"
 # Flags for one source only. The local reduce's counting atomics run in one lane and their

@@ -1,0 +1,277 @@
+// Attention over 4-bit pages for sequences with many query rows: prompts and their chunks
+// (attend.hpp has the mathematics).
+#include "attend.hpp"
+
+namespace evs {
+namespace {
+
+constexpr int kTile = 32;     // tokens taken at once
+
+// One workgroup: a share of the stages of tiles of 128 query rows (64 where NG > 4) of one KV head, a quarter of them a wave, which all take
+// every token of a stage. Every wave turns K's codes into operands for itself; V's, which take
+// twice the instructions, are turned into operands once for the four waves, a quarter by each, and
+// kept in LDS in the order in which lanes read them.
+template <int NG, bool kWhole, typename T>
+__global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a) {
+  constexpr int kTerms = QueryTerms<T>::n;
+  constexpr int kRowTiles = NG > 4 ? 1 : 2;  // of 16 rows, that a wave has
+  constexpr int VD = NG > 4 ? 2 : 1;                  // dwords of V a lane holds of a token
+  constexpr int kSubs = VD == 1 ? 4 : 2;              // 32 tokens each, of a stage
+  constexpr int kTokens = kSubs * kTile;              // of a stage
+  typedef Stage<NG, kTokens / kManyWaves, kManyWaves, kWhole> Rows;
+  __shared__ typename Rows::Lds lds;
+  __shared__ typename Rows::Tokens tk;
+  __shared__ bf16x8 s_value[kSubs][VD][8][64];
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go to the 8 XCDs in turn. Each XCD gets whole heads where they divide among the
+  // eight, whose rows then stay in its L2 from tile to tile; else a unit's heads go to one XCD.
+  uint32_t head, owner;
+  if ((a.c.heads & 7) == 0) {
+    const uint32_t at = blockIdx.x >> 3, mine = static_cast<uint32_t>(a.c.heads) >> 3;
+    head = (blockIdx.x & 7) * mine + at % mine;
+    owner = at / mine;
+  } else {
+    uint32_t outer;
+    a.heads.divmod(blockIdx.x >> 3, outer, head);
+    owner = 8 * outer + (blockIdx.x & 7);
+  }
+  // a prompt's last tiles see the most tokens: first
+  owner = a.many.workgroups - 1 - owner;
+  const char* base = a.c.base + head * a.c.sh;
+  Share share;
+  if (!find_share<true>(a, owner, kTokens, share)) return;
+  Sequence sq = sequence(a, static_cast<int>(share.seq));
+
+  while (true) {
+  const int lane = lane_now();
+  const int col = lane & 15, quad = lane >> 4;
+  const Part part = next_part<true>(a, sq, share, kTokens);
+  const int past = sq.len - sq.nq;
+  const int row0 = part.row0, last_row = part.last_row, begin = part.begin, stop = part.stop;
+  const int stages = stop > begin ? (stop - begin + kTokens - 1) / kTokens : 0;
+
+  // this wave's rows, and the tokens that some and all of them see
+  const int wave0 = row0 + 16 * kRowTiles * wave;
+  const bool any_row = wave0 <= last_row;
+  const int wave_last = min(wave0 + 16 * kRowTiles - 1, last_row);
+  const int wave_stop =
+      any_row ? min(stop, past + static_cast<int>(a.shared.div(wave_last)) + 1) : 0;
+  const int all_see =
+      any_row ? min(stop, past + static_cast<int>(a.shared.div(wave0)) + 1) : 0;
+  int sees[kRowTiles];
+  const char* qp[kRowTiles];
+#pragma unroll
+  for (int n = 0; n < kRowTiles; n++) {
+    uint32_t qi, qg;
+    a.shared.divmod(min(wave0 + 16 * n + col, last_row), qi, qg);
+    sees[n] = past + static_cast<int>(qi);
+    qp[n] = a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head;
+  }
+
+  const int32_t* table = a.tables + static_cast<int64_t>(share.seq) * a.table_stride;
+
+  f32x4 o[kRowTiles][VD][8];
+#pragma unroll
+  for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+    for (int v = 0; v < VD; v++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) o[n][v][j] = f32x4{0, 0, 0, 0};
+  Running run[kRowTiles];
+
+  if (stages > 0) {
+    Rows rows;
+    rows.place(a, wave, lane, a.one, kTokens);
+    // a page is read two stages before its rows are fetched
+    const int tid = 64 * wave + lane;
+    const auto token_of = [&](int stage) { return begin + stage * kTokens + tid; };
+    const auto page_of = [&](int stage) { return Rows::page_of(a, table, token_of(stage), stop); };
+    const auto locate = [&](int stage, int32_t page) {
+      if (64 * wave < kTokens)
+        Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, kTokens);
+    };
+    const int32_t page0 = page_of(0), page1 = page_of(1);
+    int32_t page = page_of(2);
+    locate(0, page0);
+    locate(1, page1);
+    __syncthreads();
+    rows.fetch(a, tk.at[0], lane);
+    Query<NG, T> q[kRowTiles];
+#pragma unroll
+    for (int n = 0; n < kRowTiles; n++) q[n].load(a, qp[n], quad);
+
+    // this wave's quarter of V's operands
+    const int vsub = VD == 1 ? wave : wave >> 1, vv = VD == 1 ? 0 : wave & 1;
+    const int vw = min(16 * vv + col, a.c.W - 1);
+
+    for (int i = 0; i < stages; i++) {
+      rows.store(a, lds, tk, i & 3, wave, lane);
+      __syncthreads();
+      locate(i + 2, page);
+      page = page_of(i + 3);
+      rows.fetch(a, tk.at[(i + 1) & 3], lane);
+      const int t0 = begin + i * kTokens;
+      const bool nan = __builtin_amdgcn_ballot_w64(tk.nan[i & 1][lane & (kManyWaves - 1)] != 0) != 0;
+      if (t0 + kTile * vsub < stop) {
+        Values x;
+        x.load(lds, kTile * vsub, quad, vw);
+        float sc[8];
+        x.to_f32(sc);
+        if (nan) {  // no number is added by hand below, to the rows that see it
+#pragma unroll
+          for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
+        }
+        const auto pair = [&](auto c_) {
+          constexpr int c = decltype(c_)::value;
+          bf16x8 even, odd;
+          value_pair<c>(x.codes, sc, even, odd);
+          s_value[vsub][vv][2 * c][lane] = even;
+          s_value[vsub][vv][2 * c + 1][lane] = odd;
+        };
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
+        pair(std::integral_constant<int, 2>{});
+        pair(std::integral_constant<int, 3>{});
+      }
+      __syncthreads();
+
+      // The scores of the next 32 tokens are computed beside the weights of these, so that the matrix
+      // cores and the vector units have work of each other's independence.
+      const int subs = min(max(wave_stop - t0 + kTile - 1, 0) / kTile, kSubs);
+      f32x4 acc[2][kRowTiles];
+      if (subs > 0) {
+        scores<NG, kRowTiles, T>(lds, 0, lane, a.c.W, q, acc);
+      }
+      for (int sub = 0; sub < subs; sub++) {
+        const int t = t0 + kTile * sub;
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 3][sub]);
+        float s[kRowTiles][8];
+#pragma unroll
+        for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+          for (int k = 0; k < 8; k++) s[n][k] = acc[k >> 2][n][k & 3];
+        if (t + kTile > all_see || ok != 0xFFFFFFFFu) {
+          int ahead[kRowTiles];
+#pragma unroll
+          for (int n = 0; n < kRowTiles; n++) ahead[n] = sees[n] - t - 4 * quad;
+          mask<kRowTiles>(s, ahead, ok >> (4 * quad));
+        }
+        float fade[kRowTiles];
+        if (grow<kRowTiles>(s, a.scale_log2, run, fade)) {
+#pragma unroll
+          for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+            for (int v = 0; v < VD; v++)
+#pragma unroll
+              for (int j = 0; j < 8; j++) o[n][v][j] *= fade[n];
+        }
+        if (nan) {
+#pragma unroll
+          for (int v = 0; v < VD; v++) {
+            const int grp = min(quad + 4 * v, a.c.NG - 1);
+#pragma unroll
+            for (int n = 0; n < kRowTiles; n++)
+              if (sees_nan(lds, kTile * sub, grp, sees[n] - t, ok)) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[n][v][j] += __builtin_nanf("");
+              }
+          }
+        }
+        const auto add = [&](auto more_) {
+          if (decltype(more_)::value) {
+            scores<NG, kRowTiles, T>(lds, kTile * (sub + 1), lane, a.c.W, q, acc);
+          }
+          u32x4 p[kRowTiles][kTerms];
+#pragma unroll
+          for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int v = 0; v < VD; v++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const bf16x8 x = s_value[sub][v][j][lane];
+#pragma unroll
+              for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+                for (int m = 0; m < kTerms; m++)
+                  o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      x, __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
+            }
+        };
+        if (sub + 1 < subs)
+          add(std::true_type{});
+        else
+          add(std::false_type{});
+      }
+      __syncthreads();
+    }
+  }
+
+  {
+  const int lane = lane_now();
+  const int col = lane & 15, quad = lane >> 4;
+  // Element 8 (4 quad + r) + j of row `col` of a tile is o[n][v][j][r].
+#pragma unroll
+  for (int n = 0; n < kRowTiles; n++) {
+    const float l = across_rows_sum(run[n].l);
+    const int row = wave0 + 16 * n + col;
+    if (row > last_row) continue;
+#pragma unroll
+    for (int v = 0; v < VD; v++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int w = 16 * v + 4 * quad + r;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = o[n][v][j][r];
+        if (w >= a.c.W) continue;
+        if (part.whole)
+          finish<T>(a, sq, row, head, w, x, run[n].m, l);
+        else
+          keep(a, part_row(a, a.many, owner, part.slot, head, row - row0), w, x, run[n].m, l);
+      }
+  }
+  }
+  if (share.count == 0) return;
+  next_tile<true>(a, share, sq);
+  if (share.count == 0) return;
+  }
+}
+
+template <bool kWhole, typename T>
+void launch(const AttendArgs& a, uint32_t grid, hipStream_t s) {
+  const int g = a.c.NG;
+  if (g <= 2)
+    attend_tiles<2, kWhole, T><<<grid, 64 * kManyWaves, 0, s>>>(a);
+  else if (g <= 3)
+    attend_tiles<3, kWhole, T><<<grid, 64 * kManyWaves, 0, s>>>(a);
+  else if (g <= 4)
+    attend_tiles<4, kWhole, T><<<grid, 64 * kManyWaves, 0, s>>>(a);
+  else if (g <= 6)
+    attend_tiles<6, kWhole, T><<<grid, 64 * kManyWaves, 0, s>>>(a);
+  else
+    attend_tiles<8, kWhole, T><<<grid, 64 * kManyWaves, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_type(const AttendArgs& a, uint32_t grid, hipStream_t s) {
+  if (a.c.W % 4 == 0)
+    launch<true, T>(a, grid, s);
+  else
+    launch<false, T>(a, grid, s);
+}
+
+}  // namespace
+
+int attend_many(const AttendArgs& a, int type, hipStream_t s) {
+  const uint32_t grid = a.many.workgroups * static_cast<uint32_t>(a.c.heads);
+  if (type == EVS_BF16)
+    launch_type<__bf16>(a, grid, s);
+  else
+    launch_type<_Float16>(a, grid, s);
+  EVS_LAUNCHED("evs_fp4_attend");
+  return EVS_OK;
+}
+
+}  // namespace evs
