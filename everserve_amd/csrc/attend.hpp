@@ -121,12 +121,17 @@ __device__ __forceinline__ uint32_t stages_of(const Sequence& q, uint32_t tokens
 // start of another. Each finds its share by itself from the lengths, so nothing is planned ahead of
 // the launch. Without splits the line is of whole tiles, one a share.
 //
+// A tile costs its workgroup a start (its queries, its first pages and rows) beside its stages: on
+// the line it has kStart places more, ahead of them.
+//
 // A tile in several shares is joined from their parts: the share with the tile's start keeps its
 // part in slot 1, those after it in slot 0.
 struct Share {
-  uint32_t seq, tile, first;  // the first stage of it
-  uint32_t count;             // stages
+  uint32_t seq, tile, first;  // the first place of it
+  uint32_t count;             // places
 };
+template <bool kMany>
+constexpr uint32_t kStart = kMany ? 1 : 3;  // a start took 8 to 11 us beside others, a stage 3
 
 // The fewest stages of a share, in tokens: a stage takes about 1 us where nothing else runs, and
 // the join of a split context 5 us.
@@ -150,7 +155,7 @@ __device__ __forceinline__ bool find_share(const AttendArgs& a, uint32_t at, uin
     if (s >= a.seqs) return 0;
     const Sequence q = sequence(a, s);
     tiles = tiles_of<kMany>(a, q);
-    return dealt.split ? static_cast<u64>(tiles) * stages_of(q, tokens) : tiles;
+    return dealt.split ? static_cast<u64>(tiles) * (kStart<kMany> + stages_of(q, tokens)) : tiles;
   };
   // the line's length, and the places of the first sequences, which are often all of them
   u64 total = 0, rest = 0;
@@ -220,19 +225,20 @@ __device__ __forceinline__ bool find_share(const AttendArgs& a, uint32_t at, uin
   r.seq = __builtin_amdgcn_readfirstlane(s_seq);
   if (r.seq == 0xFFFFFFFFu) return false;
   const uint32_t place = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(s_place[0]));
-  const uint32_t stages =
-      dealt.split ? stages_of(sequence(a, static_cast<int>(r.seq)), tokens) : 1;
+  const uint32_t places =
+      dealt.split ? kStart<kMany> + stages_of(sequence(a, static_cast<int>(r.seq)), tokens) : 1;
   if (kTiles) {
     r.tile = place;
     r.first = 0;
-    r.count = stages;
-    const u64 first = s_place[1] + static_cast<u64>(place) * stages;
-    const u64 head = first / share, tail = (first + stages - 1) / share;
+    r.count = places;
+    const u64 first = s_place[1] + static_cast<u64>(place) * places;
+    const u64 head = (first + (dealt.split ? kStart<kMany> : 0)) / share;
+    const u64 tail = (first + places - 1) / share;
     *owner = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(head));
     *parts = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(tail - head + 1));
   } else {
-    r.tile = place / stages;
-    r.first = place - r.tile * stages;
+    r.tile = place / places;
+    r.first = place - r.tile * places;
     const u64 left = total - start;
     r.count = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(left < share ? left : share));
   }
@@ -243,6 +249,7 @@ __device__ __forceinline__ bool find_share(const AttendArgs& a, uint32_t at, uin
 struct Part {
   int32_t row0, last_row;  // rows of the sequence
   int32_t begin, stop;     // tokens, up to the last that some row sees
+  bool none;               // no stage of it (the share ends ahead of the first)
   bool whole;              // all of the tile
   uint32_t slot;           // of the parts, if not
 };
@@ -257,12 +264,14 @@ __device__ __forceinline__ Part next_part(const AttendArgs& a, const Sequence& s
   p.last_row = min(p.row0 + (1 << bits), sq.rows) - 1;
   const int end = min(sq.len, sq.len - sq.nq + static_cast<int>(a.shared.div(p.last_row)) + 1);
   const bool split = (kMany ? a.many : a.few).split;
-  const uint32_t stages = split ? stages_of(sq, tokens) : 1;
-  const uint32_t take = min(stages - r.first, r.count);
-  p.whole = take == stages;
-  p.slot = r.first == 0 ? 1 : 0;
-  p.begin = static_cast<int>(r.first * tokens);
-  p.stop = r.first + take == stages ? end : min(end, static_cast<int>((r.first + take) * tokens));
+  const uint32_t start = split ? kStart<kMany> : 0, stages = split ? stages_of(sq, tokens) : 1;
+  const uint32_t take = min(start + stages - r.first, r.count);
+  const uint32_t from = max(r.first, start) - start, to = max(r.first + take, start) - start;
+  p.none = from == to;
+  p.whole = to - from == stages;
+  p.slot = from == 0 ? 1 : 0;
+  p.begin = static_cast<int>(from * tokens);
+  p.stop = to == stages ? end : min(end, static_cast<int>(to * tokens));
   r.count -= take;
   return p;
 }

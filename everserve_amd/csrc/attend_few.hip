@@ -45,6 +45,7 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;
   const Part part = next_part<false>(a, sq, share, tokens);
+  if (part.none) return;
   // this lane's query row, and the tokens that it sees: those up to `sees`
   uint32_t qi, qg;
   a.shared.divmod(min(part.row0 + col, part.last_row), qi, qg);

@@ -47,6 +47,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;
   const Part part = next_part<true>(a, sq, share, kTokens);
+  if (part.none) return;
   const int past = sq.len - sq.nq;
   const int row0 = part.row0, last_row = part.last_row, begin = part.begin, stop = part.stop;
   const int stages = stop > begin ? (stop - begin + kTokens - 1) / kTokens : 0;
