@@ -36,7 +36,7 @@ constexpr int many_tile(int64_t head_dim) { return head_dim > 128 ? 64 : 128; }
 
 // Tokens of a stage: what a workgroup takes at once.
 inline uint32_t few_stage(uint32_t turns) { return 32 * turns; }
-constexpr uint32_t many_stage(int64_t head_dim) { return head_dim > 128 ? 64 : 128; }
+constexpr uint32_t many_stage(int64_t head_dim) { return head_dim > 128 ? 32 : 64; }
 
 // How one kernel's work is dealt out (see Share below and `deal`).
 struct Dealt {
@@ -131,11 +131,42 @@ struct Share {
   uint32_t count;             // places
 };
 template <bool kMany>
-constexpr uint32_t kStart = kMany ? 1 : 3;  // a start took 8 to 11 us beside others, a stage 3
+constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 8 to 11 us beside others, a stage 3
 
 // The fewest stages of a share, in tokens: a stage takes about 1 us where nothing else runs, and
 // the join of a split context 5 us.
 constexpr uint32_t kMinShare = 512;
+
+// Without splits, in the kernel for many rows: row tile `at` from the sequence with the longest
+// context on, and in a sequence from the last one on, which see the most tokens. Workgroups start in
+// this order, so that the last to start have the least to do. For at most as many sequences as
+// threads.
+__device__ __forceinline__ bool longest_first(const AttendArgs& a, uint32_t at, Share& r) {
+  __shared__ int32_t s_len[64 * kManyWaves];
+  __shared__ uint32_t s_tiles[64 * kManyWaves];
+  __shared__ uint32_t s_found[2];
+  const int tid = threadIdx.x;
+  Sequence q{};
+  if (tid < a.seqs) q = sequence(a, tid);
+  const uint32_t tiles = tid < a.seqs ? tiles_of<true>(a, q) : 0;
+  s_len[tid] = q.len;
+  s_tiles[tid] = tiles;
+  if (tid == 0) s_found[0] = 0xFFFFFFFFu;
+  __syncthreads();
+  unsigned long long before = 0;
+  for (int s = 0; s < a.seqs; s++)
+    if (s_len[s] > q.len || (s_len[s] == q.len && s < tid)) before += s_tiles[s];
+  if (at >= before && at - before < tiles) {
+    s_found[0] = tid;
+    s_found[1] = tiles - 1 - static_cast<uint32_t>(at - before);
+  }
+  __syncthreads();
+  r.seq = __builtin_amdgcn_readfirstlane(s_found[0]);
+  r.tile = __builtin_amdgcn_readfirstlane(s_found[1]);
+  r.first = 0;
+  r.count = 1;
+  return r.seq != 0xFFFFFFFFu;
+}
 
 // The line's place `at` (in shares; kTiles: the start of row tile `at`), as a share. False: past its
 // end. For kTiles also how many shares the tile is in (`parts`) and the first of them (`owner`).
@@ -467,8 +498,8 @@ struct Stage {
   // Addresses of the stage's tokens' rows and whether they are tokens, ahead of the stage.
   struct Tokens {
     uint64_t at[4][kRowsOf];
-    uint32_t ok[4][kRowsOf / 32];
-    uint32_t nan[2][kWaves];  // the V rows that a wave fetched may hold a group without a number
+    uint32_t ok[8][kRowsOf / 32];
+    uint32_t nan[4][kWaves];  // the V rows that a wave fetched may hold a group without a number
   };
 
   // A chunk's token in the stage (8 bits), the dword of it in the cache from the token's first head on
@@ -533,7 +564,7 @@ struct Stage {
     for (int k = 0; k < kScaleDwords; k++) scale[k] = load_global<uint32_t>(p + 4 * k);
   }
 
-  __device__ __forceinline__ void store(const AttendArgs& a, Lds& lds, Tokens& t, int slot,
+  __device__ __forceinline__ void store(const AttendArgs& a, Lds& lds, Tokens& t, int stage,
                                         int wave, int lane) {
 #pragma unroll
     for (int j = 0; j < kLoads; j++) {
@@ -555,7 +586,7 @@ struct Stage {
     asm volatile("" : "+v"(y));
     const uint32_t row = to_of(y);
     const int kv = lane & kPairs ? 1 : 0;
-    const bool ok = (t.ok[slot][token_of(y) >> 5] >> (y & 31)) & 1;
+    const bool ok = (t.ok[stage & 7][token_of(y) >> 5] >> (y & 31)) & 1;
     bool nan = false;
 #pragma unroll
     for (int k = 0; k < kScaleDwords; k++) {
@@ -568,21 +599,21 @@ struct Stage {
         lds.scales[kv][g][row] = static_cast<uint8_t>(x >> (8 * (g & 3)));
     }
     const bool any = __builtin_amdgcn_ballot_w64(nan && kv) != 0;
-    if (lane == 0) t.nan[slot & 1][wave] = any;
+    if (lane == 0) t.nan[stage & 3][wave] = any;
   }
 
   // The page of the thread's token of a stage, read a stage before its address is needed. (No branch
   // stands around this load or those of `fetch`, or the compiler loses count of the loads under way
   // and waits for all of them.)
-  static __device__ __forceinline__ int32_t page_of(const AttendArgs& a, const int32_t* table, int t,
-                                                    int stop) {
+  static __device__ __forceinline__ int32_t page_of(const AttendArgs& a, const int32_t* table,
+                                                    uint32_t t, uint32_t stop) {
     return table[a.c.div_bs.div(min(t, stop - 1))];
   }
 
   // The tokens' addresses and flags, by as many threads.
   static __device__ __forceinline__ void locate(const AttendArgs& a, Tokens& s, int stage,
-                                                const char* base, int t, int stop, int32_t page,
-                                                uint32_t tid, uint32_t tokens) {
+                                                const char* base, uint32_t t, uint32_t stop,
+                                                int32_t page, uint32_t tid, uint32_t tokens) {
     const bool ok = tid < tokens && t < stop && page >= 0 && page < a.c.num_blocks;
     uint32_t q, off;
     a.c.div_bs.divmod(min(t, stop - 1), q, off);
@@ -590,7 +621,7 @@ struct Stage {
     if (tid < tokens) {
       s.at[stage & 3][tid] = reinterpret_cast<uint64_t>(base) +
                              (ok ? page * a.c.sb + static_cast<int64_t>(off) * a.c.so : 0);
-      if ((tid & 31) == 0) s.ok[stage & 3][tid >> 5] = static_cast<uint32_t>(flags >> (tid & 32));
+      if ((tid & 31) == 0) s.ok[stage & 7][tid >> 5] = static_cast<uint32_t>(flags >> (tid & 32));
     }
   }
 };

@@ -67,9 +67,11 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
   if (stages > 0) {
     Rows rows;
     rows.place(a, wave, lane, a.held, tokens);
-    // a page is read two stages before its rows are fetched
     const int tid = 64 * wave + lane;
-    const auto token_of = [&](int stage) { return begin + stage * tokens + tid; };
+    // (without a sign: past the last stage it may pass 2^31)
+    const auto token_of = [&](int stage) {
+      return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * tokens + tid);
+    };
     const auto page_of = [&](int stage) { return Rows::page_of(a, table, token_of(stage), stop); };
     const auto locate = [&](int stage, int32_t page) {
       if (64 * wave < tokens)
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
     // last stage the last token's page is read.)
     for (int i = 0; i < stages; i++) {
       __syncthreads();
-      rows.store(a, lds.rows[(i + 1) & 1], tk, (i + 1) & 3, wave, lane);
+      rows.store(a, lds.rows[(i + 1) & 1], tk, i + 1, wave, lane);
       locate(i + 3, page);
       page = page_of(i + 4);
       rows.fetch(a, tk.at[(i + 2) & 3], lane);
@@ -112,14 +114,14 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
         float s[1][8];
 #pragma unroll
         for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][0][k & 3];
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 3][turn]);
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][turn]);
         const bool whole = t + kTile <= all_see && ok == 0xFFFFFFFFu;
         bool nan = false;
         if (!whole) {
           const int ahead[1] = {sees - t - 4 * quad};
           mask<1>(s, ahead, ok >> (4 * quad));
           nan = __builtin_amdgcn_ballot_w64(
-                    tk.nan[i & 1][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
+                    tk.nan[i & 3][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
         }
         float fade[1];
         if (grow<1>(s, a.scale_log2, run, fade)) {

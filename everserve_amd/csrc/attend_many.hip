@@ -7,21 +7,21 @@ namespace {
 
 constexpr int kTile = 32;     // tokens taken at once
 
-// One workgroup: a share of the stages of tiles of 128 query rows (64 where NG > 4) of one KV head, a quarter of them a wave, which all take
-// every token of a stage. Every wave turns K's codes into operands for itself; V's, which take
-// twice the instructions, are turned into operands once for the four waves, a quarter by each, and
-// kept in LDS in the order in which lanes read them.
+// One workgroup: a share of the stages of tiles of 128 query rows (64 where NG > 4) of one KV head, a
+// quarter of them a wave, which all take every token of a stage. Every wave turns K's codes into
+// operands for itself; V's, which take twice the instructions, are turned into operands once for the
+// four waves, a quarter by each, a stage ahead, and kept in LDS in the order in which lanes read them.
 template <int NG, bool kWhole, typename T>
 __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a) {
   constexpr int kTerms = QueryTerms<T>::n;
   constexpr int kRowTiles = NG > 4 ? 1 : 2;  // of 16 rows, that a wave has
   constexpr int VD = NG > 4 ? 2 : 1;                  // dwords of V a lane holds of a token
-  constexpr int kSubs = VD == 1 ? 4 : 2;              // 32 tokens each, of a stage
+  constexpr int kSubs = VD == 1 ? 2 : 1;              // 32 tokens each, of a stage
   constexpr int kTokens = kSubs * kTile;              // of a stage
   typedef Stage<NG, kTokens / kManyWaves, kManyWaves, kWhole> Rows;
-  __shared__ typename Rows::Lds lds;
+  __shared__ typename Rows::Lds lds[3];
   __shared__ typename Rows::Tokens tk;
-  __shared__ bf16x8 s_value[kSubs][VD][8][64];
+  __shared__ bf16x8 s_value[2][kSubs][VD][8][64];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the 8 XCDs in turn. Each XCD gets whole heads where they divide among the
@@ -36,11 +36,11 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
     a.heads.divmod(blockIdx.x >> 3, outer, head);
     owner = 8 * outer + (blockIdx.x & 7);
   }
-  // a prompt's last tiles see the most tokens: first
-  owner = a.many.workgroups - 1 - owner;
   const char* base = a.c.base + head * a.c.sh;
   Share share;
-  if (!find_share<true>(a, owner, kTokens, share)) return;
+  if (!(a.many.split || a.seqs > 64 * kManyWaves ? find_share<true>(a, owner, kTokens, share)
+                                                 : longest_first(a, owner, share)))
+    return;
   Sequence sq = sequence(a, static_cast<int>(share.seq));
 
   while (true) {
@@ -84,69 +84,89 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
   if (stages > 0) {
     Rows rows;
     rows.place(a, wave, lane, a.one, kTokens);
-    // a page is read two stages before its rows are fetched
     const int tid = 64 * wave + lane;
-    const auto token_of = [&](int stage) { return begin + stage * kTokens + tid; };
+    // (without a sign: past the last stage it may pass 2^31)
+    const auto token_of = [&](int stage) {
+      return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * kTokens + tid);
+    };
     const auto page_of = [&](int stage) { return Rows::page_of(a, table, token_of(stage), stop); };
     const auto locate = [&](int stage, int32_t page) {
       if (64 * wave < kTokens)
         Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, kTokens);
     };
-    const int32_t page0 = page_of(0), page1 = page_of(1);
-    int32_t page = page_of(2);
-    locate(0, page0);
-    locate(1, page1);
+    int32_t pages[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) pages[k] = page_of(k);
+    int32_t page = page_of(4);
+#pragma unroll
+    for (int k = 0; k < 4; k++) locate(k, pages[k]);
     __syncthreads();
+    Rows second = rows;
     rows.fetch(a, tk.at[0], lane);
+    second.fetch(a, tk.at[1], lane);
     Query<NG, T> q[kRowTiles];
 #pragma unroll
     for (int n = 0; n < kRowTiles; n++) q[n].load(a, qp[n], quad);
 
-    // this wave's quarter of V's operands
-    const int vsub = VD == 1 ? wave : wave >> 1, vv = VD == 1 ? 0 : wave & 1;
+    // this wave's quarter of V's operands: half of the elements of a dword of 32 tokens
+    const int vsub = VD == 1 ? wave >> 1 : 0, vv = VD == 1 ? 0 : wave >> 1;
     const int vw = min(16 * vv + col, a.c.W - 1);
-
-    for (int i = 0; i < stages; i++) {
-      rows.store(a, lds, tk, i & 3, wave, lane);
-      __syncthreads();
-      locate(i + 2, page);
-      page = page_of(i + 3);
-      rows.fetch(a, tk.at[(i + 1) & 3], lane);
-      const int t0 = begin + i * kTokens;
-      const bool nan = __builtin_amdgcn_ballot_w64(tk.nan[i & 1][lane & (kManyWaves - 1)] != 0) != 0;
-      if (t0 + kTile * vsub < stop) {
-        Values x;
-        x.load(lds, kTile * vsub, quad, vw);
-        float sc[8];
-        x.to_f32(sc);
-        if (nan) {  // no number is added by hand below, to the rows that see it
+    const auto any_nan = [&](int stage) {
+      return __builtin_amdgcn_ballot_w64(tk.nan[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
+    };
+    const auto convert = [&](int stage, int at) {
+      Values x;
+      x.load(lds[at], kTile * vsub, quad, vw);
+      float sc[8];
+      x.to_f32(sc);
+      if (any_nan(stage)) {  // no number is added by hand below, to the rows that see it
 #pragma unroll
-          for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
-        }
-        const auto pair = [&](auto c_) {
-          constexpr int c = decltype(c_)::value;
-          bf16x8 even, odd;
-          value_pair<c>(x.codes, sc, even, odd);
-          s_value[vsub][vv][2 * c][lane] = even;
-          s_value[vsub][vv][2 * c + 1][lane] = odd;
-        };
-        pair(std::integral_constant<int, 0>{});
-        pair(std::integral_constant<int, 1>{});
+        for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
+      }
+      auto* to = &s_value[stage & 1][vsub][vv];
+      const auto pair = [&](auto c_) {
+        constexpr int c = decltype(c_)::value;
+        bf16x8 even, odd;
+        value_pair<c>(x.codes, sc, even, odd);
+        (*to)[2 * c][lane] = even;
+        (*to)[2 * c + 1][lane] = odd;
+      };
+      if (wave & 1) {
         pair(std::integral_constant<int, 2>{});
         pair(std::integral_constant<int, 3>{});
+      } else {
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
       }
-      __syncthreads();
+    };
+    rows.store(a, lds[0], tk, 0, wave, lane);
+    second.store(a, lds[1], tk, 1, wave, lane);
+    rows.fetch(a, tk.at[2], lane);
+    __syncthreads();
+    convert(0, 0);
 
-      // The scores of the next 32 tokens are computed beside the weights of these, so that the matrix
-      // cores and the vector units have work of each other's independence.
+    // Stage i is computed with while the values of the next are converted, the rows of the one after
+    // are written to LDS and those of a third are on their way: one barrier a stage. (Past the last
+    // stage the last token's page is read.)
+    int now = 0, ahead1 = 1, ahead2 = 2;  // where the stages' rows lie in LDS
+    for (int i = 0; i < stages; i++) {
+      __syncthreads();
+      rows.store(a, lds[ahead2], tk, i + 2, wave, lane);
+      locate(i + 4, page);
+      page = page_of(i + 5);
+      rows.fetch(a, tk.at[(i + 3) & 3], lane);
+      convert(i + 1, ahead1);
+      const bool nan = any_nan(i);
+      const int t0 = begin + i * kTokens;
+
       const int subs = min(max(wave_stop - t0 + kTile - 1, 0) / kTile, kSubs);
       f32x4 acc[2][kRowTiles];
       if (subs > 0) {
-        scores<NG, kRowTiles, T>(lds, 0, lane, a.c.W, q, acc);
+        scores<NG, kRowTiles, T>(lds[now], 0, lane, a.c.W, q, acc);
       }
       for (int sub = 0; sub < subs; sub++) {
         const int t = t0 + kTile * sub;
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 3][sub]);
+        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][sub]);
         float s[kRowTiles][8];
 #pragma unroll
         for (int n = 0; n < kRowTiles; n++)
@@ -173,40 +193,43 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
             const int grp = min(quad + 4 * v, a.c.NG - 1);
 #pragma unroll
             for (int n = 0; n < kRowTiles; n++)
-              if (sees_nan(lds, kTile * sub, grp, sees[n] - t, ok)) {
+              if (sees_nan(lds[now], kTile * sub, grp, sees[n] - t, ok)) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) o[n][v][j] += __builtin_nanf("");
               }
           }
         }
-        const auto add = [&](auto more_) {
-          if (decltype(more_)::value) {
-            scores<NG, kRowTiles, T>(lds, kTile * (sub + 1), lane, a.c.W, q, acc);
-          }
-          u32x4 p[kRowTiles][kTerms];
+        u32x4 p[kRowTiles][kTerms];
 #pragma unroll
-          for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
+        for (int v = 0; v < VD; v++) {
+          // all reads are under way before the weights are computed and the first product waits
+          bf16x8 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[j] = s_value[i & 1][sub][v][j][lane];
           __builtin_amdgcn_sched_barrier(0);
+          if (v == 0) {
 #pragma unroll
-          for (int v = 0; v < VD; v++)
+            for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
+          }
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const bf16x8 x = s_value[sub][v][j][lane];
+          for (int j = 0; j < 8; j++)
 #pragma unroll
-              for (int n = 0; n < kRowTiles; n++)
+            for (int n = 0; n < kRowTiles; n++)
 #pragma unroll
-                for (int m = 0; m < kTerms; m++)
-                  o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                      x, __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
-            }
-        };
+              for (int m = 0; m < kTerms; m++)
+                o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    x[j], __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
+        }
+        // the next tokens' codes are converted while the matrix cores have these
         if (sub + 1 < subs)
-          add(std::true_type{});
-        else
-          add(std::false_type{});
+          scores<NG, kRowTiles, T>(lds[now], kTile * (sub + 1), lane, a.c.W, q, acc);
       }
-      __syncthreads();
+      const int free = now;
+      now = ahead1;
+      ahead1 = ahead2;
+      ahead2 = free;
     }
+    __syncthreads();  // the rows and values have been read
   }
 
   {
