@@ -199,6 +199,123 @@ __global__ __launch_bounds__(kPlanThreads) void plan_emit(PlanArgs a) {
   }
 }
 
+// The bitmap and its counts by one workgroup, in LDS; for small tables and caches the whole plan
+// (kWhole). A launch costs about 2 us here and 3 on the host: the plan of 2,304 entries and 2,048
+// pages took 11 us in four launches and takes 6 in this one. Emitting by one workgroup is slower
+// from about 4,096 entries on (13,568 entries and 16,384 pages: 28 us against 13).
+constexpr uint32_t kOneWords = 4096;  // 131,072 pages
+constexpr int64_t kOneEntries = 1 << 15;
+constexpr uint32_t kWholeWords = 512;
+constexpr int64_t kWholeEntries = 1 << 12;
+
+template <bool kWhole>
+__global__ __launch_bounds__(kScanThreads) void plan_one(PlanArgs a, FastDiv width) {
+  __shared__ uint32_t s_bitmap[kWhole ? kWholeWords : kOneWords];
+  __shared__ uint32_t s_before[kWholeWords];
+  __shared__ uint32_t s_wave[kScanThreads / 64];
+  constexpr uint32_t kPer = kWhole ? 1 : kOneWords / kScanThreads;  // words a thread counts
+  constexpr int kAtOnce = 4;                           // entries a thread reads at once
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t entries = static_cast<uint32_t>(a.entries);
+  for (uint32_t w = tid; w < a.words; w += kScanThreads) s_bitmap[w] = 0;
+  __syncthreads();
+  const auto read = [&](uint32_t i0, int32_t (&id)[kAtOnce], bool (&used)[kAtOnce]) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++) {
+      const uint32_t i = i0 + k * kScanThreads;
+      used[k] = false;
+      if (i < entries) {
+        uint32_t row, col;
+        width.divmod(i, row, col);
+        id[k] = a.tables[row * a.row_stride + col];
+        const uint32_t held = a.counts == nullptr ? a.width
+                                                  : static_cast<uint32_t>(max(a.counts[row], 0));
+        used[k] = col < held && id[k] >= 0 && id[k] < a.num_blocks;
+      }
+    }
+  };
+  for (uint32_t i0 = tid; i0 < entries; i0 += kAtOnce * kScanThreads) {
+    int32_t id[kAtOnce];
+    bool used[kAtOnce];
+    read(i0, id, used);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++)
+      if (used[k]) atomicOr(&s_bitmap[id[k] >> 5], 1u << (id[k] & 31));
+  }
+  __syncthreads();
+  // used pages before each word
+  uint32_t count[kPer], mine = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; k++) {
+    const uint32_t w = kPer * tid + k;
+    count[k] = w < a.words ? __popc(s_bitmap[w]) : 0;
+    mine += count[k];
+  }
+  uint32_t sum = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = __shfl_up(sum, d);
+    if (lane >= static_cast<uint32_t>(d)) sum += up;
+  }
+  if (lane == 63) s_wave[wave] = sum;
+  __syncthreads();
+  uint32_t before = sum - mine, u = 0;
+  for (uint32_t k = 0; k < kScanThreads / 64; k++) {
+    if (k < wave) before += s_wave[k];
+    u += s_wave[k];
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kPer; k++) {
+    const uint32_t w = kPer * tid + k;
+    if (w < a.words) {
+      if (kWhole) {
+        s_before[w] = before;
+      } else {
+        a.before[w] = before;
+        a.bitmap[w] = s_bitmap[w];
+      }
+    }
+    before += count[k];
+  }
+  if (!kWhole) {
+    if (tid == 0) a.sizes[0] = static_cast<int32_t>(u);
+    return;
+  }
+  __syncthreads();
+  PlanArgs b = a;
+  b.bitmap = s_bitmap;
+  b.before = s_before;
+  const uint32_t stay = u < static_cast<uint32_t>(a.num_blocks) ? used_before(b, u) : u;
+  const uint32_t moved = u - stay;
+  if (tid == 0) {
+    a.sizes[0] = static_cast<int32_t>(u);
+    a.sizes[1] = static_cast<int32_t>(moved);
+  }
+  for (uint32_t id = tid; id < static_cast<uint32_t>(a.num_blocks); id += kScanThreads) {
+    const bool used = (s_bitmap[id >> 5] >> (id & 31)) & 1;
+    if (used != (id >= u)) continue;
+    const uint32_t at = used_before(b, id);
+    if (used)
+      a.src[at - stay] = static_cast<int32_t>(id);
+    else
+      a.dst[id - at] = static_cast<int32_t>(id);
+  }
+  for (int64_t i = moved + tid; i < a.room; i += kScanThreads) a.src[i] = a.dst[i] = -1;
+  for (uint32_t i0 = tid; i0 < entries; i0 += kAtOnce * kScanThreads) {
+    int32_t id[kAtOnce];
+    bool used[kAtOnce];
+    read(i0, id, used);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; k++) {
+      const uint32_t i = i0 + k * kScanThreads;
+      if (i >= entries) continue;
+      if (used[k] && static_cast<uint32_t>(id[k]) >= u)
+        id[k] = free_page(b, used_before(b, static_cast<uint32_t>(id[k])) - stay);
+      a.tables_out[i] = id[k];
+    }
+  }
+}
+
 uint32_t grid_of(int64_t items, int64_t most) {
   const int64_t g = (items + kPlanThreads - 1) / kPlanThreads;
   return static_cast<uint32_t>(g < 1 ? 1 : g < most ? g : most);
@@ -364,16 +481,24 @@ extern "C" int evs_plan_compaction(const int32_t* tables, int64_t rows, int64_t 
   a.bitmap = static_cast<uint32_t*>(workspace);
   a.before = a.bitmap + a.words;
   const hipStream_t s = evs::as_stream(stream);
-  if (a.words > 0) {
+  if (a.words <= evs::kWholeWords && a.entries <= evs::kWholeEntries) {
+    evs::plan_one<true><<<1, evs::kScanThreads, 0, s>>>(a, evs::FastDiv(a.width));
+    EVS_LAUNCHED(who);
+    return EVS_OK;
+  }
+  if (a.words <= evs::kOneWords && a.entries <= evs::kOneEntries) {
+    evs::plan_one<false><<<1, evs::kScanThreads, 0, s>>>(a, evs::FastDiv(a.width));
+    EVS_LAUNCHED(who);
+  } else {
     evs::plan_clear<<<evs::grid_of(a.words, 256), evs::kPlanThreads, 0, s>>>(a);
     EVS_LAUNCHED(who);
     if (a.entries > 0) {
       evs::plan_mark<<<evs::grid_of(a.entries, 2048), evs::kPlanThreads, 0, s>>>(a);
       EVS_LAUNCHED(who);
     }
+    evs::plan_scan<<<1, evs::kScanThreads, 0, s>>>(a);
+    EVS_LAUNCHED(who);
   }
-  evs::plan_scan<<<1, evs::kScanThreads, 0, s>>>(a);
-  EVS_LAUNCHED(who);
   const int64_t items = a.entries > num_blocks ? a.entries : num_blocks;
   evs::plan_emit<<<evs::grid_of(items, 2048), evs::kPlanThreads, 0, s>>>(a);
   EVS_LAUNCHED(who);

@@ -301,6 +301,11 @@ _TWO = ctypes.c_int64 * 2
 _HERE = contextlib.nullcontext()
 
 
+def _five(strides):
+    """Five strides as the library takes them: as they are where a caller keeps them converted."""
+    return strides if type(strides) is _FIVE else _FIVE(*strides)
+
+
 def _stream_of(device) -> int:
     """The handle of torch's current stream of ``device``, a ``torch.device`` of a GPU."""
     import torch
@@ -359,6 +364,7 @@ class Kernels:
         self.MAX_ROWS, self.CTRL_WORDS, self.ABORT, self.LATE, self.BOUND = (int(w) for w in words)
         self._workspace: dict = {}  # order_pairs' workspace, per (device, stream)
         self._pairs: dict = {}  # scatter_rows' sorted pairs, per (device, stream)
+        self._attend_bytes: dict = {}  # fp4_attend's workspace sizes, by its counts
 
     def _check(self, rc: int) -> None:
         if rc != EVS_OK:
@@ -744,28 +750,28 @@ class Kernels:
         import torch
 
         types = _row_types()
-        if key.dim() != 3 or key.shape != value.shape or slots.numel() != key.shape[0]:
+        shape, dtype = key.shape, key.dtype
+        if len(shape) != 3 or shape != value.shape or slots.numel() != shape[0]:
             raise RuntimeError(f"fp4_write_rows: {slots.numel()} slots, keys of shape "
                                f"{tuple(key.shape)} and values of {tuple(value.shape)}")
-        if key.dtype != value.dtype or key.dtype not in types:
+        if dtype != value.dtype or dtype not in types:
             raise RuntimeError(f"fp4_write_rows: rows of {key.dtype} and {value.dtype}: both must "
                                "be bf16, f16 or f32")
         if not (key.is_cuda and value.is_cuda and cache.is_cuda):
             raise RuntimeError("fp4_write_rows: the rows and the cache must be on the device")
-        n, heads, d = key.shape
+        n, heads, d = shape
         ks, vs = key.stride(), value.stride()
         if ks[2] != 1 or vs[2] != 1:
             raise RuntimeError("fp4_write_rows: a row's elements must be contiguous")
         sp = _device_ptr(slots, "fp4_write_rows: slots", torch.long)
         _one_device("fp4_write_rows", key, value, slots, cache)
         with _on_device_of(cache):
-            self._check(
-                self._lib.evs_fp4_write_rows(
-                    key.data_ptr(), value.data_ptr(), _FOUR(ks[0], ks[1], vs[0], vs[1]),
-                    types[key.dtype], sp, n, cache.data_ptr(), num_blocks, block_size, heads, d,
-                    _FIVE(*strides), _stream_of(cache.device),
-                )
-            )
+            rc = self._lib.evs_fp4_write_rows(
+                key.data_ptr(), value.data_ptr(), _FOUR(ks[0], ks[1], vs[0], vs[1]), types[dtype],
+                sp, n, cache.data_ptr(), num_blocks, block_size, heads, d, _five(strides),
+                _stream_of(cache.device))
+        if rc != EVS_OK:
+            self._check(rc)
 
     def fp4_read_rows(self, cache, num_blocks: int, block_size: int, heads: int, d: int,
                       strides: Sequence[int], slots, dtype):
@@ -782,15 +788,15 @@ class Kernels:
         sp = _device_ptr(slots, "fp4_read_rows: slots", torch.long)
         _one_device("fp4_read_rows", cache, slots)
         n = slots.numel()
-        key = torch.empty((n, heads, d), dtype=dtype, device=cache.device)
-        value = torch.empty((n, heads, d), dtype=dtype, device=cache.device)
+        device = cache.device
+        # one allocation: half the host time of two
+        key, value = torch.empty((2, n, heads, d), dtype=dtype, device=device).unbind(0)
         with _on_device_of(cache):
-            self._check(
-                self._lib.evs_fp4_read_rows(
-                    cache.data_ptr(), num_blocks, block_size, heads, d, _FIVE(*strides), sp, n,
-                    key.data_ptr(), value.data_ptr(), types[dtype], _stream_of(cache.device),
-                )
-            )
+            rc = self._lib.evs_fp4_read_rows(
+                cache.data_ptr(), num_blocks, block_size, heads, d, _five(strides), sp, n,
+                key.data_ptr(), value.data_ptr(), types[dtype], _stream_of(device))
+        if rc != EVS_OK:
+            self._check(rc)
         return key, value
 
     def fp4_attend(self, q, cache, num_blocks: int, block_size: int, heads: int,
@@ -845,24 +851,27 @@ class Kernels:
         if return_lse:
             lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
         _one_device("fp4_attend", q, cache, block_tables, seq_lens, q_starts, out)
-        need = ctypes.c_int64()
+        max_len = max_len or width * block_size
+        counts = (seqs, tokens, q_heads, heads, d, max_q, max_len)
         with _on_device_of(q):
-            self._check(self._lib.evs_fp4_attend_workspace(
-                seqs, tokens, q_heads, heads, d, max_q, max_len or width * block_size,
-                ctypes.byref(need)))
-            work = None
-            if need.value:
-                work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-            self._check(
-                self._lib.evs_fp4_attend(
-                    q.data_ptr(), _TWO(qs[0], qs[1]), type_, out.data_ptr(),
-                    lse.data_ptr() if return_lse else None, tokens, q_heads, cache.data_ptr(),
-                    num_blocks, block_size, heads, d, _FIVE(*strides), block_tables.data_ptr(),
-                    block_tables.stride(0), width, lp, starts or None, seqs, max_q,
-                    max_len or width * block_size, d ** -0.5 if scale is None else scale,
-                    work.data_ptr() if need.value else None, need.value, _stream_of(q.device),
-                )
-            )
+            need = self._attend_bytes.get(counts)
+            if need is None:
+                size = ctypes.c_int64()
+                self._check(self._lib.evs_fp4_attend_workspace(*counts, ctypes.byref(size)))
+                if len(self._attend_bytes) >= 4096:  # the same counts come back in a serving loop
+                    self._attend_bytes.clear()
+                need = self._attend_bytes[counts] = size.value
+            device = q.device
+            work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            rc = self._lib.evs_fp4_attend(
+                q.data_ptr(), _TWO(qs[0], qs[1]), type_, out.data_ptr(),
+                lse.data_ptr() if return_lse else None, tokens, q_heads, cache.data_ptr(),
+                num_blocks, block_size, heads, d, _five(strides), block_tables.data_ptr(),
+                block_tables.stride(0), width, lp, starts or None, seqs, max_q, max_len,
+                d ** -0.5 if scale is None else scale, work.data_ptr() if need else None, need,
+                _stream_of(device))
+        if rc != EVS_OK:
+            self._check(rc)
         return (out, lse) if return_lse else out
 
     # -------------------------------------------------------------- pages of a cache
@@ -886,13 +895,11 @@ class Kernels:
             raise RuntimeError(f"copy_blocks: one count, not {count.numel()}")
         _one_device("copy_blocks", layer_ptrs, src, dst, count)
         with _on_device_of(src):
-            self._check(
-                self._lib.evs_copy_blocks(
-                    lp, layer_ptrs.numel(), sp, dp, src.numel(), cp, int(num_blocks), int(heads),
-                    int(d), int(block_size), _FIVE(*strides), int(elem_size),
-                    _stream_of(src.device),
-                )
-            )
+            rc = self._lib.evs_copy_blocks(
+                lp, layer_ptrs.numel(), sp, dp, src.numel(), cp, int(num_blocks), int(heads),
+                int(d), int(block_size), _five(strides), int(elem_size), _stream_of(src.device))
+        if rc != EVS_OK:
+            self._check(rc)
 
     def plan_compaction(self, block_tables, counts, num_blocks: int):
         """The moves that pack the pages that ``block_tables`` (int32 [rows, width], of row r the

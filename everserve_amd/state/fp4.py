@@ -14,6 +14,8 @@ The reference has no counterpart: its caches are its engine's, at 8 bits or more
 
 from __future__ import annotations
 
+import ctypes
+
 from everserve_amd.state.paged import CacheLayout, PagedKV, strides_of
 
 GROUP = 32
@@ -81,6 +83,7 @@ class Fp4Cache:
         if self.strides[4] != 1 or any(x % 4 for x in self.strides[:4]):
             raise ValueError(f"a half-row's bytes must be contiguous and start on 4 bytes: strides "
                              f"{self.strides}")
+        self._strides = (ctypes.c_int64 * 5)(*self.strides)  # converted once for every call
 
     @classmethod
     def empty(cls, num_blocks: int, block_size: int, heads: int, head_dim: int,
@@ -96,17 +99,18 @@ class Fp4Cache:
         """Round ``key`` and ``value`` ([n, heads, head_dim]) to 4 bits and write them at ``slots``
         (int64 [n], distinct; a slot outside the cache is padding). One launch on the current
         stream."""
-        if key.dim() != 3 or tuple(key.shape[1:]) != (self.num_heads, self.head_dim):
+        shape = key.shape
+        if len(shape) != 3 or shape[1] != self.num_heads or shape[2] != self.head_dim:
             raise ValueError(f"write: rows of shape {tuple(key.shape)}, expected "
                              f"[n, {self.num_heads}, {self.head_dim}]")
         _kernels().fp4_write_rows(key, value, slots, self.tensor, self.num_blocks, self.block_size,
-                                  self.strides)
+                                  self._strides)
 
     def read(self, slots, dtype):
         """``(key, value)`` [n, heads, head_dim] of ``dtype`` at ``slots`` (int64 [n]); zeros for a
         slot outside the cache. One launch on the current stream."""
         return _kernels().fp4_read_rows(self.tensor, self.num_blocks, self.block_size,
-                                        self.num_heads, self.head_dim, self.strides, slots, dtype)
+                                        self.num_heads, self.head_dim, self._strides, slots, dtype)
 
     def attend(self, q, block_tables, seq_lens, q_starts=None, max_q: int | None = None,
                scale: float | None = None, max_len: int = 0, out=None, return_lse: bool = False):
@@ -116,7 +120,7 @@ class Fp4Cache:
             raise ValueError(f"attend: queries of shape {tuple(q.shape)}, expected "
                              f"[tokens, heads, {self.head_dim}]")
         return _kernels().fp4_attend(q, self.tensor, self.num_blocks, self.block_size,
-                                     self.num_heads, self.strides, block_tables, seq_lens,
+                                     self.num_heads, self._strides, block_tables, seq_lens,
                                      q_starts, max_q, scale, max_len, out, return_lse)
 
 

@@ -12,6 +12,7 @@ The reference leaves pages to its engine and has no counterpart.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 from typing import Sequence
 
@@ -76,6 +77,7 @@ class PageMover:
                 t.data_ptr() % 16 for t in layers):
             raise ValueError("caches with strides of whole 16-byte words must start on one")
         self._layers = list(layers)  # the table holds their addresses
+        self._strides = (ctypes.c_int64 * 5)(*self.strides)  # converted once for every call
         self._ptrs = torch.tensor([t.data_ptr() for t in layers], dtype=torch.long,
                                   device=first.device)
 
@@ -85,7 +87,7 @@ class PageMover:
         nothing; destinations must be distinct, and none a pair's source. One launch on the
         current stream."""
         _kernels().copy_blocks(self._ptrs, src, dst, self.num_blocks, self.num_heads,
-                               self.head_dim, self.block_size, self.strides, self.elem, count)
+                               self.head_dim, self.block_size, self._strides, self.elem, count)
 
     def plan(self, block_tables, counts=None) -> Compaction:
         """The moves that pack the pages that ``block_tables`` name (int32 [rows, width], of row r
