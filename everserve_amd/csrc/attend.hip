@@ -8,21 +8,35 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 
-// Rows of a row tile that was split, joined: workgroups for each row tile and head, which take the
-// tile's rows in turn. A workgroup's threads are dealt a dword of elements each and, as many times over
-// as there are parts for, the parts in turn; the rest of them takes further rows.
+// Rows of a row tile that was split, joined: workgroups for each row tile that there may be and head,
+// which take the tile's rows in turn. A workgroup's threads are dealt a dword of elements each and, as
+// many times over as there are parts for, the parts in turn; the rest of them takes further rows.
+//
+// A launch of its own (about 6 us): joined by the last of a tile's workgroups to end instead, a decode
+// step took 113 us for 86, with parts that pass the caches, and 417 with fences of the GPU's scope.
 template <bool kMany, typename T>
-__global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a, uint32_t tokens) {
+__global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a) {
   __shared__ float s_v[kJoinThreads][8 + 1];
   __shared__ float s_m[kJoinThreads];
   __shared__ float s_l[kJoinThreads];
   const Dealt& dealt = kMany ? a.many : a.few;
-  uint32_t head, tile;
-  a.heads.divmod(blockIdx.x, tile, head);
-  Share at;
+  uint32_t head, at, seq, tile;
+  a.heads.divmod(blockIdx.x, at, head);
+  const uint4 in = dealt.tiles_in[at];
   uint32_t owner, parts;
-  if (!find_share<kMany, true>(a, tile, tokens, at, &owner, &parts) || parts == 1) return;
-  const Sequence sq = sequence(a, static_cast<int>(at.seq));
+  if (kMany) {
+    if (in.z < 2) return;
+    seq = __builtin_amdgcn_readfirstlane(in.x);
+    tile = __builtin_amdgcn_readfirstlane(in.y);
+    owner = at;
+    parts = __builtin_amdgcn_readfirstlane(in.z);
+  } else {
+    dealt.most.divmod(at, seq, tile);
+    owner = __builtin_amdgcn_readfirstlane(in.x);
+    parts = __builtin_amdgcn_readfirstlane(in.y);
+  }
+  const Sequence sq = sequence_of_all(a, seq);
+  if (!kMany && (tile >= tiles_of<kMany>(a, sq) || parts == 1)) return;  // no tile: `in` is garbage
   // threads: [row][turn][dword], a row's dwords rounded up to a power of two
   const uint32_t lanes = 1u << a.join_bits;
   uint32_t turn_bits = 0;
@@ -32,7 +46,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a, uint32_
   const uint32_t w = threadIdx.x & (lanes - 1), turn = (threadIdx.x >> a.join_bits) & (turns - 1);
   const uint32_t mine = threadIdx.x >> (a.join_bits + turn_bits);
   const uint32_t wr = min(w, static_cast<uint32_t>(a.c.W) - 1);
-  const uint32_t held = min(1 << dealt.tile_bits, sq.rows - static_cast<int>(at.tile << dealt.tile_bits));  // rows of it
+  const uint32_t held = min(1 << dealt.tile_bits, sq.rows - static_cast<int>(tile << dealt.tile_bits));  // rows of it
   for (uint32_t r0 = blockIdx.y * rows; r0 < held; r0 += gridDim.y * rows) {
     const uint32_t r = r0 + mine;
     const int row = static_cast<int>(min(r, held - 1));
@@ -70,23 +84,25 @@ __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a, uint32_
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] += s_v[t][j] * f;
     }
-    finish<T>(a, sq, static_cast<int>((at.tile << dealt.tile_bits) + r), head, w, v, top, total);
+    finish<T>(a, sq, static_cast<int>((tile << dealt.tile_bits) + r), head, w, v, top, total);
   }
 }
 
 template <bool kMany>
-int join(const AttendArgs& a, int type, uint32_t tokens, hipStream_t s) {
+int join(const AttendArgs& a, int type, hipStream_t s) {
   const Dealt& dealt = kMany ? a.many : a.few;
   const uint32_t rows = static_cast<uint32_t>(dealt.rows);
-  const uint32_t across = dealt.tiles * static_cast<uint32_t>(a.c.heads);
+  const uint32_t heads = static_cast<uint32_t>(a.c.heads);
+  const uint32_t across =
+      (kMany ? dealt.workgroups : static_cast<uint32_t>(a.seqs) * dealt.most.d) * heads;
   // a workgroup a row where there are few tiles
-  uint32_t down = 1024 / across;
+  uint32_t down = (kMany ? 4096 : 1024) / across;
   down = down < 1 ? 1 : down > rows ? rows : down;
   const dim3 grid(across, down);
   if (type == EVS_BF16)
-    join_parts<kMany, __bf16><<<grid, kJoinThreads, 0, s>>>(a, tokens);
+    join_parts<kMany, __bf16><<<grid, kJoinThreads, 0, s>>>(a);
   else
-    join_parts<kMany, _Float16><<<grid, kJoinThreads, 0, s>>>(a, tokens);
+    join_parts<kMany, _Float16><<<grid, kJoinThreads, 0, s>>>(a);
   EVS_LAUNCHED("evs_fp4_attend");
   return EVS_OK;
 }
@@ -103,18 +119,29 @@ struct Deal {
   int64_t few_bytes, many_bytes;  // of the parts' workspace
 };
 
-// `tiles`: row tiles that there may be; `groups`: workgroups that share a place in the line.
-void deal_tiles(Dealt& r, int64_t& bytes, int64_t tiles, int64_t rows, int64_t groups, int64_t heads,
-                int64_t d, int64_t max_len, int64_t at_once) {
-  r.split = tiles * groups < 4 * at_once && max_len > 2 * kMinShare;
+// `tiles`: row tiles that there may be, `most` of one sequence; `in`: entries of tiles_in (0: one a
+// workgroup); `groups`: workgroups that share a place in the line.
+void deal_tiles(Dealt& r, int64_t& bytes, int64_t tiles, int64_t most, int64_t in, int64_t rows,
+                int64_t groups, int64_t heads, int64_t d, int64_t max_len, int64_t at_once) {
+  // (more sequences and heads than 2^24 leave no context to split)
+  r.split = tiles * groups < 4 * at_once && max_len > 2 * kMinShare &&
+            in * heads < (int64_t{1} << 24);
   int64_t workgroups = r.split ? at_once / groups : tiles;
   workgroups = workgroups < 1 ? 1 : workgroups;
   workgroups = (workgroups + 7) / 8 * 8;
-  const int64_t most = int64_t{1} << 30;  // more are refused by the caller
-  r.workgroups = static_cast<uint32_t>(workgroups < most ? workgroups : most);
-  r.tiles = static_cast<uint32_t>(tiles < most ? tiles : most);
+  const int64_t bound = int64_t{1} << 30;  // more are refused by the caller
+  r.workgroups = static_cast<uint32_t>(workgroups < bound ? workgroups : bound);
   r.rows = static_cast<int32_t>(rows);
-  bytes = r.split ? (workgroups * 2 * heads * rows * (d + 2) * 4 + 15) / 16 * 16 : 0;
+  if (r.split) {
+    r.most = FastDiv(static_cast<uint32_t>(most));
+    r.in = in > 0 ? in : workgroups;
+    bytes = r.in * 16 + (workgroups * 2 * heads * rows * (d + 2) * 4 + 15) / 16 * 16;
+  }
+}
+
+void place_parts(Dealt& r, void* at) {
+  r.tiles_in = static_cast<uint4*>(at);
+  r.part = reinterpret_cast<float*>(static_cast<char*>(at) + r.in * 16);
 }
 
 Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d, int64_t max_q,
@@ -124,8 +151,8 @@ Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d
   const int64_t rows = max_q * shared;
   // row tiles: a sequence's rows, rounded up
   if (shared <= kFewRows) {
-    int64_t tiles = (least(rows, kFewRows) + kFewTile - 1) / kFewTile * seqs;
-    tiles = least(tiles, tokens * shared / kFewTile + seqs);
+    const int64_t most = (least(rows, kFewRows) + kFewTile - 1) / kFewTile;
+    const int64_t tiles = least(most * seqs, tokens * shared / kFewTile + seqs);
     // The most heads, up to the waves, that leave shares for all workgroups: heads that lie side by
     // side share memory lines (8 of 128: 5.4 TB/s, in fours 4.4 and in twos 3.2), but the more of
     // them a workgroup has, the fewer tokens its waves take at once.
@@ -134,15 +161,15 @@ Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d
     for (int64_t n = 2; side_by_side && n <= kFewWaves; n++)
       if (heads % n == 0 && shares * (heads / n) >= few_at_once(d)) r.held = static_cast<uint32_t>(n);
     r.few.tile_bits = 4;
-    deal_tiles(r.few, r.few_bytes, tiles, least(rows, kFewTile), heads / r.held, heads, d,
+    deal_tiles(r.few, r.few_bytes, tiles, most, most * seqs, least(rows, kFewTile), heads / r.held, heads, d,
                max_len, few_at_once(d));
   }
   if (rows > kFewRows) {
     const int64_t tile = many_tile(d);
-    int64_t tiles = (rows + tile - 1) / tile * seqs;
-    tiles = least(tiles, tokens * shared / tile + seqs);
+    const int64_t most = (rows + tile - 1) / tile;
+    const int64_t tiles = least(most * seqs, tokens * shared / tile + seqs);
     r.many.tile_bits = tile == 64 ? 6 : 7;
-    deal_tiles(r.many, r.many_bytes, tiles, least(rows, tile), heads, heads, d, max_len,
+    deal_tiles(r.many, r.many_bytes, tiles, most, 0, least(rows, tile), heads, heads, d, max_len,
                kManyAtOnce);
   }
   return r;
@@ -232,8 +259,8 @@ extern "C" int evs_fp4_attend(const void* q, const int64_t* q_strides, int type,
   const bool side_by_side = strides[2] > 0 && strides[2] <= 2 * evs::fp4_row_bytes(head_dim);
   const evs::Deal deal =
       evs::deal(seqs, tokens, shared, heads, head_dim, max_q, max_len, side_by_side);
-  const int64_t tiles = (static_cast<int64_t>(deal.few.tiles) + deal.few.workgroups +
-                         deal.many.tiles + deal.many.workgroups) * heads;
+  const int64_t tiles =
+      (static_cast<int64_t>(deal.few.workgroups) + deal.many.workgroups) * heads;
   EVS_REQUIRE(tiles < (int64_t{1} << 24), "%s: %lld tiles of query rows: below 2^24", who,
               static_cast<long long>(tiles));
   const int64_t need = deal.few_bytes + deal.many_bytes;
@@ -244,8 +271,10 @@ extern "C" int evs_fp4_attend(const void* q, const int64_t* q_strides, int type,
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   a.few = deal.few;
   a.many = deal.many;
-  a.few.part = static_cast<float*>(workspace);
-  a.many.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + deal.few_bytes);
+  if (need > 0) {
+    evs::place_parts(a.few, workspace);
+    evs::place_parts(a.many, static_cast<char*>(workspace) + deal.few_bytes);
+  }
   const uint32_t held = deal.held > 0 ? deal.held : 1;
   a.held = evs::FastDiv(held);
   a.turns = evs::kFewWaves / held;
@@ -255,12 +284,12 @@ extern "C" int evs_fp4_attend(const void* q, const int64_t* q_strides, int type,
   if (a.few.workgroups > 0) {
     if (const int rc = evs::attend_few(a, type, s)) return rc;
     if (a.few.split)
-      if (const int rc = evs::join<false>(a, type, evs::few_stage(a.turns), s)) return rc;
+      if (const int rc = evs::join<false>(a, type, s)) return rc;
   }
   if (a.many.workgroups > 0) {
     if (const int rc = evs::attend_many(a, type, s)) return rc;
     if (a.many.split)
-      if (const int rc = evs::join<true>(a, type, evs::many_stage(head_dim), s)) return rc;
+      if (const int rc = evs::join<true>(a, type, s)) return rc;
   }
   return EVS_OK;
 }

@@ -41,11 +41,16 @@ constexpr uint32_t many_stage(int64_t head_dim) { return head_dim > 128 ? 32 : 6
 // How one kernel's work is dealt out (see Share below and `deal`).
 struct Dealt {
   uint32_t workgroups;  // a KV head (few: a group of them) has, a multiple of 8
-  uint32_t tiles;       // row tiles a KV head may have
   bool split;           // contexts may be split between workgroups
   uint32_t tile_bits;   // log2 of a tile's rows
   int32_t rows;         // of them that are ever used
   float* part;  // [workgroups, 2, heads, rows, d + 2]: a part's sums, running maximum and total
+  // Which shares a split tile is in, for the join. few: [seqs, tiles a sequence may have], the first
+  // and how many (tiles of 16 rows are many, but few of a sequence); many: [workgroups], of the share
+  // with the tile's start, the sequence, the tile and how many, below 2 if there is none.
+  uint4* tiles_in;
+  int64_t in;    // entries of it
+  FastDiv most;  // tiles that a sequence may have
 };
 
 struct AttendArgs {
@@ -97,11 +102,28 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int s) {
   return r;
 }
 
+// The sequence of a whole workgroup, in scalars.
+__device__ __forceinline__ Sequence sequence_of_all(const AttendArgs& a, uint32_t s) {
+  Sequence r = sequence(a, static_cast<int>(s));
+  r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
+  r.nq = __builtin_amdgcn_readfirstlane(r.nq);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
+  r.rows = __builtin_amdgcn_readfirstlane(r.rows);
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
   return v;
+}
+
+// A value that all lanes have alike, as a scalar.
+__device__ __forceinline__ unsigned long long scalar(unsigned long long v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return static_cast<unsigned long long>(hi) << 32 | lo;
 }
 
 // Row tiles of a sequence in the kernel for many rows, or in that for few.
@@ -129,6 +151,7 @@ __device__ __forceinline__ uint32_t stages_of(const Sequence& q, uint32_t tokens
 struct Share {
   uint32_t seq, tile, first;  // the first place of it
   uint32_t count;             // places
+  unsigned long long line, size;  // the tile's start on the line, places of a share
 };
 template <bool kMany>
 constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 8 to 11 us beside others, a stage 3
@@ -168,111 +191,79 @@ __device__ __forceinline__ bool longest_first(const AttendArgs& a, uint32_t at, 
   return r.seq != 0xFFFFFFFFu;
 }
 
-// The line's place `at` (in shares; kTiles: the start of row tile `at`), as a share. False: past its
-// end. For kTiles also how many shares the tile is in (`parts`) and the first of them (`owner`).
-template <bool kMany, bool kTiles = false>
+// Share `at` of the line. False: past its end.
+template <bool kMany>
 __device__ __forceinline__ bool find_share(const AttendArgs& a, uint32_t at, uint32_t tokens,
-                                           Share& r, uint32_t* owner = nullptr,
-                                           uint32_t* parts = nullptr) {
+                                           Share& r) {
   typedef unsigned long long u64;
-  __shared__ u64 s_wave[2][kFewWaves];
-  __shared__ u64 s_place[2];
-  __shared__ uint32_t s_seq;
+  __shared__ u64 s_wave[kFewWaves];
+  __shared__ uint32_t s_seq, s_place;
   const Dealt& dealt = kMany ? a.many : a.few;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int threads = blockDim.x, waves = threads >> 6;
-  const auto length = [&](int s, uint32_t& tiles) -> u64 {
-    tiles = 0;
+  const auto length = [&](int s) -> u64 {
     if (s >= a.seqs) return 0;
     const Sequence q = sequence(a, s);
-    tiles = tiles_of<kMany>(a, q);
+    const uint32_t tiles = tiles_of<kMany>(a, q);
     return dealt.split ? static_cast<u64>(tiles) * (kStart<kMany> + stages_of(q, tokens)) : tiles;
   };
   // the line's length, and the places of the first sequences, which are often all of them
-  u64 total = 0, rest = 0;
-  uint32_t tiles;
-  u64 mine = length(tid, tiles);
+  u64 total = 0;
+  u64 mine = length(tid);
   if (a.seqs > threads) {
-    uint32_t unused;
-    for (int s = tid + threads; s < a.seqs; s += threads) rest += length(s, unused);
+    u64 rest = 0;
+    for (int s = tid + threads; s < a.seqs; s += threads) rest += length(s);
     rest = wave_sum(rest);
-    if (lane == 0) s_wave[1][wave] = rest;
+    if (lane == 0) s_wave[wave] = rest;
     __syncthreads();
-    for (int k = 0; k < waves; k++) total += s_wave[1][k];
+    for (int k = 0; k < waves; k++) total += s_wave[k];
   }
   if (tid == 0) s_seq = 0xFFFFFFFFu;
-  u64 start = 0, share = 1;
-  u64 before = 0, tiles_before = 0;
+  u64 start = 0, before = 0;
+  r.size = 1;
   for (int s0 = 0; s0 < a.seqs; s0 += threads) {
-    if (s0 > 0) mine = length(s0 + tid, tiles);
-    u64 sum = mine, t_sum = tiles;
+    if (s0 > 0) mine = length(s0 + tid);
+    u64 sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const u64 up = __shfl_up(sum, d);
       if (lane >= d) sum += up;
-      if (kTiles) {
-        const u64 t_up = __shfl_up(t_sum, d);
-        if (lane >= d) t_sum += t_up;
-      }
     }
     __syncthreads();
-    if (lane == 63) {
-      s_wave[0][wave] = sum;
-      if (kTiles) s_wave[1][wave] = t_sum;
-    }
+    if (lane == 63) s_wave[wave] = sum;
     __syncthreads();
-    u64 from = before + sum - mine, t_from = tiles_before + t_sum - tiles;
+    u64 from = before + sum - mine;
     for (int k = 0; k < waves; k++) {
-      if (k < wave) from += s_wave[0][k];
-      before += s_wave[0][k];
-      if (kTiles) {
-        if (k < wave) t_from += s_wave[1][k];
-        tiles_before += s_wave[1][k];
-      }
+      if (k < wave) from += s_wave[k];
+      before += s_wave[k];
     }
     if (s0 == 0) {
-      total += before;
+      total = scalar(total + before);
       if (dealt.split) {
         const u64 least = (kMinShare + tokens - 1) / tokens;
-        share = (total + dealt.workgroups - 1) / dealt.workgroups;
-        share = share < least ? least : share;
+        r.size = (total + dealt.workgroups - 1) / dealt.workgroups;
+        r.size = scalar(r.size < least ? least : r.size);
       }
-      start = at * share;
-      if (!kTiles && start >= total) return false;  // uniform
+      start = at * r.size;
+      if (start >= total) return false;  // uniform
     }
-    if (kTiles) {
-      if (at >= t_from && at - t_from < tiles) {
-        s_seq = s0 + tid;
-        s_place[0] = at - t_from;
-        s_place[1] = from;
-      }
-    } else if (start >= from && start - from < mine) {
+    if (start >= from && start - from < mine) {
       s_seq = s0 + tid;
-      s_place[0] = start - from;
+      s_place = static_cast<uint32_t>(start - from);
     }
-    if (kTiles ? at < tiles_before : start < before) break;
+    if (start < before) break;
   }
   __syncthreads();
   r.seq = __builtin_amdgcn_readfirstlane(s_seq);
   if (r.seq == 0xFFFFFFFFu) return false;
-  const uint32_t place = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(s_place[0]));
+  const uint32_t place = __builtin_amdgcn_readfirstlane(s_place);
   const uint32_t places =
-      dealt.split ? kStart<kMany> + stages_of(sequence(a, static_cast<int>(r.seq)), tokens) : 1;
-  if (kTiles) {
-    r.tile = place;
-    r.first = 0;
-    r.count = places;
-    const u64 first = s_place[1] + static_cast<u64>(place) * places;
-    const u64 head = (first + (dealt.split ? kStart<kMany> : 0)) / share;
-    const u64 tail = (first + places - 1) / share;
-    *owner = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(head));
-    *parts = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(tail - head + 1));
-  } else {
-    r.tile = place / places;
-    r.first = place - r.tile * places;
-    const u64 left = total - start;
-    r.count = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(left < share ? left : share));
-  }
+      dealt.split ? kStart<kMany> + stages_of(sequence_of_all(a, r.seq), tokens) : 1;
+  r.tile = place / places;
+  r.first = place - r.tile * places;
+  r.line = scalar(start - r.first);
+  const u64 left = total - start;
+  r.count = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(left < r.size ? left : r.size));
   return true;
 }
 
@@ -282,6 +273,7 @@ struct Part {
   int32_t begin, stop;     // tokens, up to the last that some row sees
   bool none;               // no stage of it (the share ends ahead of the first)
   bool whole;              // all of the tile
+  uint32_t places;         // of the tile
   uint32_t slot;           // of the parts, if not
 };
 
@@ -299,6 +291,7 @@ __device__ __forceinline__ Part next_part(const AttendArgs& a, const Sequence& s
   const uint32_t take = min(start + stages - r.first, r.count);
   const uint32_t from = max(r.first, start) - start, to = max(r.first + take, start) - start;
   p.none = from == to;
+  p.places = start + stages;
   p.whole = to - from == stages;
   p.slot = from == 0 ? 1 : 0;
   p.begin = static_cast<int>(from * tokens);
@@ -310,12 +303,14 @@ __device__ __forceinline__ Part next_part(const AttendArgs& a, const Sequence& s
 // On to the next tile, of the next sequence that has one (there is one while the share's count is
 // above zero).
 template <bool kMany>
-__device__ __forceinline__ void next_tile(const AttendArgs& a, Share& r, Sequence& sq) {
+__device__ __forceinline__ void next_tile(const AttendArgs& a, const Part& p, Share& r,
+                                          Sequence& sq) {
   r.first = 0;
+  r.line += p.places;
   if (++r.tile < tiles_of<kMany>(a, sq)) return;
   r.tile = 0;
   while (static_cast<int>(++r.seq) < a.seqs) {
-    sq = sequence(a, static_cast<int>(r.seq));
+    sq = sequence_of_all(a, r.seq);
     if (tiles_of<kMany>(a, sq) > 0) return;
   }
   r.count = 0;
@@ -327,6 +322,17 @@ __device__ __forceinline__ int lane_now() {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));
   return lane;
+}
+
+// The kernel's arguments, read afresh, for the same reason: what a part's start and end need of them is
+// not to take the stages' scalar registers.
+__device__ __forceinline__ AttendArgs args_now() {
+  uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  AttendArgs a;
+  __builtin_memcpy(&a, (const void*)reinterpret_cast<const __attribute__((address_space(4))) char*>(p),
+                   sizeof(a));
+  return a;
 }
 
 // bf16 terms that a query, and a weight for such a query's output, is the sum of.
@@ -743,7 +749,7 @@ __device__ __forceinline__ void finish(const AttendArgs& a, const Sequence& sq, 
     a.lse[at] = total == 0 ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
-// Where a part's row of a head lies.
+// Where a part's row of a head lies; such rows start on 8 bytes.
 __device__ __forceinline__ float* part_row(const AttendArgs& a, const Dealt& dealt, uint32_t owner,
                                            uint32_t slot, uint32_t head, int r) {
   return dealt.part + ((static_cast<int64_t>(owner) * 2 + slot) * a.c.heads + head) *
@@ -759,6 +765,21 @@ __device__ __forceinline__ void keep(const AttendArgs& a, float* part, int w, co
     part[a.c.d] = top;
     part[a.c.d + 1] = total;
   }
+}
+
+// For the join, by one thread of the share with the tile's start.
+template <bool kMany>
+__device__ __forceinline__ void describe(const AttendArgs& a, const Share& r, uint32_t owner,
+                                         const Part& p) {
+  const Dealt& dealt = kMany ? a.many : a.few;
+  const uint32_t first = static_cast<uint32_t>((r.line + kStart<kMany>) / r.size);
+  const uint32_t last = static_cast<uint32_t>((r.line + p.places - 1) / r.size);
+  const uint32_t parts = last - first + 1;
+  if (kMany)
+    dealt.tiles_in[owner] = make_uint4(r.seq, r.tile, parts, 0);
+  else
+    dealt.tiles_in[static_cast<int64_t>(r.seq) * dealt.most.d + r.tile] =
+        make_uint4(first, parts, 0, 0);
 }
 
 int attend_few(const AttendArgs& a, int type, hipStream_t s);

@@ -38,14 +38,18 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
   const int tokens = kTile * a.turns;  // of a stage
   const char* base = a.c.base + static_cast<int64_t>(group * held) * a.c.sh;
   Share share;
-  if (!find_share<false>(a, owner, tokens, share)) return;
-  Sequence sq = sequence(a, static_cast<int>(share.seq));
+  if (!find_share<false>(args_now(), owner, tokens, share)) return;
+  Sequence sq = sequence_of_all(a, share.seq);
 
   while (true) {
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;
-  const Part part = next_part<false>(a, sq, share, tokens);
+  const Part part = next_part<false>(args_now(), sq, share, tokens);
   if (part.none) return;
+  if (part.slot == 1 && group == 0 && threadIdx.x == 0) {
+    const AttendArgs b = args_now();
+    if (b.few.split) describe<false>(b, share, owner, part);
+  }
   // this lane's query row, and the tokens that it sees: those up to `sees`
   uint32_t qi, qg;
   a.shared.divmod(min(part.row0 + col, part.last_row), qi, qg);
@@ -171,16 +175,18 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
   run[0].l = across_rows_sum(run[0].l);
 
   {
+  const AttendArgs b = args_now();
+  const uint32_t held = b.held.d;
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;
   // Element 8 (4 quad + r) + j of row `col` is o[v][j][r].
   const auto put = [&](uint32_t at, int r, int w, const float (&x)[8], float top, float total) {
     if (part.whole)
-      finish<T>(a, sq, part.row0 + r, at, w, x, top, total);
+      finish<T>(b, sq, part.row0 + r, at, w, x, top, total);
     else
-      keep(a, part_row(a, a.few, owner, part.slot, at, r), w, x, top, total);
+      keep(b, part_row(b, b.few, owner, part.slot, at, r), w, x, top, total);
   };
-  if (a.turns == 1) {
+  if (b.turns == 1) {
     if (part.row0 + col <= part.last_row) {
 #pragma unroll
       for (int v = 0; v < VD; v++)
@@ -190,7 +196,7 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) x[j] = o[v][j][r];
-          if (w < a.c.W) put(head, col, w, x, run[0].m, run[0].l);
+          if (w < b.c.W) put(head, col, w, x, run[0].m, run[0].l);
         }
     }
   } else {
@@ -206,18 +212,18 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
       lds.joined.l[wave][col] = run[0].l;
     }
     __syncthreads();
-    const int W = a.c.W;
+    const int W = b.c.W;
     for (uint32_t x = threadIdx.x; x < kFewTile * held * W; x += blockDim.x) {
       const int rh = x / W, w = x - rh * W;
       uint32_t r_, hh;
-      a.held.divmod(rh, r_, hh);
+      b.held.divmod(rh, r_, hh);
       const int r = r_;
       if (part.row0 + r > part.last_row) break;  // rows ascend
       float top = -INFINITY;
-      for (uint32_t k = hh; k < held * a.turns; k += held) top = fmaxf(top, lds.joined.m[k][r]);
+      for (uint32_t k = hh; k < held * b.turns; k += held) top = fmaxf(top, lds.joined.m[k][r]);
       const float ref = top == -INFINITY ? 0.0f : top;
       float total = 0, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (uint32_t k = hh; k < held * a.turns; k += held) {
+      for (uint32_t k = hh; k < held * b.turns; k += held) {
         const float f = __builtin_amdgcn_exp2f(lds.joined.m[k][r] - ref);
         total += f * lds.joined.l[k][r];
 #pragma unroll
@@ -228,9 +234,9 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
   }
   }
   if (share.count == 0) return;
-  next_tile<false>(a, share, sq);
+  next_tile<false>(args_now(), part, share, sq);
   if (share.count == 0) return;
-  __syncthreads();  // the joined rows have been read
+  __syncthreads();  // LDS is free
   }
 }
 

@@ -37,17 +37,21 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
     owner = 8 * outer + (blockIdx.x & 7);
   }
   const char* base = a.c.base + head * a.c.sh;
+  if (a.many.split && head == 0 && threadIdx.x == 0)
+    a.many.tiles_in[owner] = make_uint4(0, 0, 0, 0);
   Share share;
   if (!(a.many.split || a.seqs > 64 * kManyWaves ? find_share<true>(a, owner, kTokens, share)
                                                  : longest_first(a, owner, share)))
     return;
-  Sequence sq = sequence(a, static_cast<int>(share.seq));
+  Sequence sq = sequence_of_all(a, share.seq);
 
   while (true) {
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;
   const Part part = next_part<true>(a, sq, share, kTokens);
   if (part.none) return;
+  if (part.slot == 1 && !part.whole && head == 0 && threadIdx.x == 0)
+    describe<true>(a, share, owner, part);
   const int past = sq.len - sq.nq;
   const int row0 = part.row0, last_row = part.last_row, begin = part.begin, stop = part.stop;
   const int stages = stop > begin ? (stop - begin + kTokens - 1) / kTokens : 0;
@@ -258,8 +262,9 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
   }
   }
   if (share.count == 0) return;
-  next_tile<true>(a, share, sq);
+  next_tile<true>(a, part, share, sq);
   if (share.count == 0) return;
+  __syncthreads();  // LDS is free
   }
 }
 
