@@ -16,8 +16,7 @@ struct RowsIo {
   int64_t n;
   uint32_t units;     // work items of this launch
   FastDiv per_token;  // items a token has
-  FastDiv per_half;   // items a half-row has
-  FastDiv heads;
+  FastDiv per_half;   // items a head's row has
   bool vector;  // rows may be read in 16-byte words
 };
 
@@ -65,48 +64,58 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 // next would be 8, so up to 7 the largest element is off by no more than half a step, as the
 // others are. (2^126 is left out because 4 times it is no finite bf16.) Codes are rounded to the
 // nearest, ties to even, by the hardware's conversion.
+//
+// K's group and V's at the same place are one work item: they share the index arithmetic, and both
+// their loads are under way before the first is needed.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void write_rows(RowsIo a) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t unit = u >> 2, lane = u & 3;
   if (unit >= a.units) return;  // whole groups of four lanes leave
-  uint32_t token, rest, half, g, kv, h;
+  uint32_t token, rest, h, g;
   a.per_token.divmod(unit, token, rest);
-  a.per_half.divmod(rest, half, g);
-  a.heads.divmod(half, kv, h);
+  a.per_half.divmod(rest, h, g);
   const int64_t slot = a.slots[token];
   const uint32_t w = 4 * g + lane;  // this lane's dword of codes
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (w < static_cast<uint32_t>(a.c.W))
-    load8<T>(a.in[kv] + token * a.in_token[kv] + h * a.in_head[kv] + w * (8 * sizeof(T)), a.vector,
-             x);
-  char* row = half_row(a.c, slot, h, kv);
-  // magnitudes compare as their bits do, an infinity and a NaN above every number
-  uint32_t most = 0;
+  const bool in = w < static_cast<uint32_t>(a.c.W);
+  float x[2][8] = {};
+  if (in) {
 #pragma unroll
-  for (int j = 0; j < 8; j++)
-    most = max(most, __builtin_bit_cast(uint32_t, x[j]) & 0x7FFFFFFFu);
-  most = quad_max(most);
-  const bool number = most < 0x7F800000u;
-  // the exponent, and one more where the mantissa is above 1.75: 7 = 1.75 * 4
-  const int e = static_cast<int>((most + 0x1FFFFFu) >> 23) - 2;
-  const uint32_t byte = number ? static_cast<uint32_t>(min(max(e, 1), 252)) : kScaleNaN;
-  uint32_t codes = 0;
-  if (number) {
-    const float s = scale_of(byte);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], s, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], s, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], s, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], s, 3);
+    for (int kv = 0; kv < 2; kv++)
+      load8<T>(a.in[kv] + token * a.in_token[kv] + h * a.in_head[kv] + w * (8 * sizeof(T)),
+               a.vector, x[kv]);
   }
-  if (row == nullptr) return;
-  if (w < static_cast<uint32_t>(a.c.W)) reinterpret_cast<uint32_t*>(row)[w] = codes;
-  uint8_t* scales = reinterpret_cast<uint8_t*>(row + 4 * a.c.W);
-  if (lane == 0) scales[g] = static_cast<uint8_t>(byte);
-  // zeros after the last scale, up to a multiple of four bytes
-  const uint32_t tail = a.c.NG & 3;
-  if (lane > 0 && g == static_cast<uint32_t>(a.c.NG) - 1 && tail != 0 && lane <= 4 - tail)
-    scales[a.c.NG + lane - 1] = 0;
+  char* row = half_row(a.c, slot, h, 0);
+#pragma unroll
+  for (int kv = 0; kv < 2; kv++) {
+    // magnitudes compare as their bits do, an infinity and a NaN above every number
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      most = max(most, __builtin_bit_cast(uint32_t, x[kv][j]) & 0x7FFFFFFFu);
+    most = quad_max(most);
+    const bool number = most < 0x7F800000u;
+    // the exponent, and one more where the mantissa is above 1.75: 7 = 1.75 * 4
+    const int e = static_cast<int>((most + 0x1FFFFFu) >> 23) - 2;
+    const uint32_t byte = number ? static_cast<uint32_t>(min(max(e, 1), 252)) : kScaleNaN;
+    uint32_t codes = 0;
+    if (number) {
+      const float s = scale_of(byte);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[kv][0], x[kv][1], s, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[kv][2], x[kv][3], s, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[kv][4], x[kv][5], s, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[kv][6], x[kv][7], s, 3);
+    }
+    if (row == nullptr) continue;
+    char* half = row + kv * a.c.skv;
+    if (in) reinterpret_cast<uint32_t*>(half)[w] = codes;
+    uint8_t* scales = reinterpret_cast<uint8_t*>(half + 4 * a.c.W);
+    if (lane == 0) scales[g] = static_cast<uint8_t>(byte);
+    // zeros after the last scale, up to a multiple of four bytes
+    const uint32_t tail = a.c.NG & 3;
+    if (lane > 0 && g == static_cast<uint32_t>(a.c.NG) - 1 && tail != 0 && lane <= 4 - tail)
+      scales[a.c.NG + lane - 1] = 0;
+  }
 }
 
 template <typename T>
@@ -114,27 +123,32 @@ __device__ __forceinline__ T from_f32(float v) {
   return static_cast<T>(v);
 }
 
-// One lane turns a dword of codes into eight elements.
+// One lane turns a dword of K's codes and the one of V's at the same place into eight elements each.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void read_rows(RowsIo a) {
   const uint32_t unit = blockIdx.x * kThreads + threadIdx.x;
   if (unit >= a.units) return;
-  uint32_t token, rest, half, w, kv, h;
+  uint32_t token, rest, h, w;
   a.per_token.divmod(unit, token, rest);
-  a.per_half.divmod(rest, half, w);
-  a.heads.divmod(half, kv, h);
-  const char* row = half_row(a.c, a.slots[token], h, kv);
-  T v[8];
-  if (row == nullptr) {
+  a.per_half.divmod(rest, h, w);
+  const char* row = half_row(a.c, a.slots[token], h, 0);
+  uint32_t codes[2] = {0, 0};
+  float s[2] = {1.0f, 1.0f};
+  if (row != nullptr) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = from_f32<T>(0.0f);
-  } else {
-    const uint32_t codes = reinterpret_cast<const uint32_t*>(row)[w];
-    const float s = scale_of(reinterpret_cast<const uint8_t*>(row)[4 * a.c.W + (w >> 2)]);
-    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0);
-    const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1);
-    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2);
-    const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3);
+    for (int kv = 0; kv < 2; kv++) {
+      const char* half = row + kv * a.c.skv;
+      codes[kv] = reinterpret_cast<const uint32_t*>(half)[w];
+      s[kv] = scale_of(reinterpret_cast<const uint8_t*>(half)[4 * a.c.W + (w >> 2)]);
+    }
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; kv++) {
+    const f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[kv], s[kv], 0);
+    const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[kv], s[kv], 1);
+    const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[kv], s[kv], 2);
+    const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[kv], s[kv], 3);
+    T v[8];
     v[0] = from_f32<T>(p0[0]);
     v[1] = from_f32<T>(p0[1]);
     v[2] = from_f32<T>(p1[0]);
@@ -143,10 +157,9 @@ __global__ __launch_bounds__(kThreads) void read_rows(RowsIo a) {
     v[5] = from_f32<T>(p2[1]);
     v[6] = from_f32<T>(p3[0]);
     v[7] = from_f32<T>(p3[1]);
+    char* out = a.out[kv] + static_cast<int64_t>(unit) * static_cast<int64_t>(8 * sizeof(T));
+    __builtin_memcpy(__builtin_assume_aligned(out, 16), v, sizeof(v));
   }
-  char* out = a.out[kv] + ((static_cast<int64_t>(token) * a.c.heads + h) * a.c.W + w) *
-                              static_cast<int64_t>(8 * sizeof(T));
-  __builtin_memcpy(__builtin_assume_aligned(out, 16), v, sizeof(v));
 }
 
 // Work items are counted in 32 bits: a longer list goes in several launches.
@@ -216,10 +229,9 @@ extern "C" int evs_fp4_write_rows(const void* key, const void* value, const int6
   }
   a.slots = slots;
   a.n = n;
-  const int64_t per_token = 2 * heads * a.c.NG;
+  const int64_t per_token = heads * a.c.NG;
   a.per_token = evs::FastDiv(static_cast<uint32_t>(per_token));
   a.per_half = evs::FastDiv(static_cast<uint32_t>(a.c.NG));
-  a.heads = evs::FastDiv(static_cast<uint32_t>(heads));
   const hipStream_t s = evs::as_stream(stream);
   return evs::in_launches(a, per_token, 4, [&](const evs::RowsIo& b, uint32_t grid) {
     if (type == EVS_BF16)
@@ -253,10 +265,9 @@ extern "C" int evs_fp4_read_rows(const void* cache, int64_t num_blocks, int64_t 
   a.in_token[0] = a.in_token[1] = heads * head_dim * evs::elem_bytes(type);
   a.slots = slots;
   a.n = n;
-  const int64_t per_token = 2 * heads * a.c.W;
+  const int64_t per_token = heads * a.c.W;
   a.per_token = evs::FastDiv(static_cast<uint32_t>(per_token));
   a.per_half = evs::FastDiv(static_cast<uint32_t>(a.c.W));
-  a.heads = evs::FastDiv(static_cast<uint32_t>(heads));
   const hipStream_t s = evs::as_stream(stream);
   return evs::in_launches(a, per_token, 1, [&](const evs::RowsIo& b, uint32_t grid) {
     if (type == EVS_BF16)
