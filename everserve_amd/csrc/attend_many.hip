@@ -118,12 +118,12 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
     const auto any_nan = [&](int stage) {
       return __builtin_amdgcn_ballot_w64(tk.nan[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
     };
-    const auto convert = [&](int stage, int at) {
+    const auto convert = [&](int stage, int at, bool nan) {
       Values x;
       x.load(lds[at], kTile * vsub, quad, vw);
       float sc[8];
       x.to_f32(sc);
-      if (any_nan(stage)) {  // no number is added by hand below, to the rows that see it
+      if (nan) {  // no number is added by hand below, to the rows that see it
 #pragma unroll
         for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
       }
@@ -147,28 +147,30 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
     second.store(a, lds[1], tk, 1, wave, lane);
     rows.fetch(a, tk.at[2], lane);
     __syncthreads();
-    convert(0, 0);
+    convert(0, 0, any_nan(0));
 
     // Stage i is computed with while the values of the next are converted, the rows of the one after
     // are written to LDS and those of a third are on their way: one barrier a stage. (Past the last
     // stage the last token's page is read.)
     int now = 0, ahead1 = 1, ahead2 = 2;  // where the stages' rows lie in LDS
+    bool nan = false, nan_next = any_nan(0);
+    f32x4 first[2][kRowTiles];
+    scores<NG, kRowTiles, T>(lds[0], 0, lane, a.c.W, q, first);
     for (int i = 0; i < stages; i++) {
       __syncthreads();
       rows.store(a, lds[ahead2], tk, i + 2, wave, lane);
       locate(i + 4, page);
       page = page_of(i + 5);
       rows.fetch(a, tk.at[(i + 3) & 3], lane);
-      convert(i + 1, ahead1);
-      const bool nan = any_nan(i);
+      nan = nan_next;
+      nan_next = any_nan(i + 1);
+      convert(i + 1, ahead1, nan_next);
       const int t0 = begin + i * kTokens;
 
-      const int subs = min(max(wave_stop - t0 + kTile - 1, 0) / kTile, kSubs);
-      f32x4 acc[2][kRowTiles];
-      if (subs > 0) {
-        scores<NG, kRowTiles, T>(lds[now], 0, lane, a.c.W, q, acc);
-      }
-      for (int sub = 0; sub < subs; sub++) {
+      // 32 tokens, whose scores are in `acc`; those of the next 32 go to `after`, beside the products
+      // with the values: their codes are converted while the matrix cores have these.
+      const auto take = [&](int sub, f32x4 (&acc)[2][kRowTiles], int rows_after, int at_after,
+                            f32x4 (&after)[2][kRowTiles]) {
         const int t = t0 + kTile * sub;
         const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][sub]);
         float s[kRowTiles][8];
@@ -224,9 +226,17 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
                 o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                     x[j], __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
         }
-        // the next tokens' codes are converted while the matrix cores have these
-        if (sub + 1 < subs)
-          scores<NG, kRowTiles, T>(lds[now], kTile * (sub + 1), lane, a.c.W, q, acc);
+        scores<NG, kRowTiles, T>(lds[rows_after], at_after, lane, a.c.W, q, after);
+      };
+      if (t0 < wave_stop) {
+        if (kSubs == 1) {
+          take(0, first, ahead1, 0, first);
+        } else {
+          f32x4 second_half[2][kRowTiles];
+          take(0, first, now, kTile, second_half);
+          if (t0 + kTile < wave_stop)
+            take(1, second_half, ahead1, 0, first);
+        }
       }
       const int free = now;
       now = ahead1;
