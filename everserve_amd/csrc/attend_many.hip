@@ -217,6 +217,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
 #pragma unroll
             for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
           }
+          __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int j = 0; j < 8; j++)
 #pragma unroll
@@ -227,6 +228,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
                     x[j], __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
         }
         scores<NG, kRowTiles, T>(lds[rows_after], at_after, lane, a.c.W, q, after);
+        __builtin_amdgcn_s_setprio(0);
       };
       if (t0 < wave_stop) {
         if (kSubs == 1) {
