@@ -109,7 +109,7 @@ int join(const AttendArgs& a, int type, hipStream_t s) {
 
 // Workgroups of a kernel that the GPU holds at once: shares are made for so many, to end together.
 constexpr int64_t kCus = 256;
-int64_t few_at_once(int64_t d) { return (d > 128 ? 1 : 2) * kCus; }
+int64_t few_at_once(int64_t d) { return (d > 64 ? 1 : 2) * kCus; }
 constexpr int64_t kManyAtOnce = 2 * kCus;
 
 // How a call's work is dealt out, from its counts alone (the lengths are on the device).

@@ -11,9 +11,11 @@ constexpr int kTile = 32;  // tokens a wave takes at once
 // side. A stage is 32 tokens of every wave's head; waves with one head take a stage's tokens in
 // turns of 32 and join their results in LDS.
 template <int NG, bool kWhole, typename T>
-__global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(AttendArgs a) {
+__global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(AttendArgs a) {
   constexpr int kTerms = QueryTerms<T>::n;
   constexpr int VD = NG > 4 ? 2 : 1;  // dwords of V a lane holds of a token
+  // stages whose rows are on their way; wide rows leave no registers for a second
+  constexpr int kAhead = NG > 4 ? 1 : 2;
   typedef Stage<NG, kTile, kFewWaves, kWhole> Rows;
   struct Joined {
     float o[kFewWaves][kFewTile][128 * VD + 4];
@@ -81,12 +83,16 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
       if (64 * wave < tokens)
         Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, tokens);
     };
-    const int32_t page0 = page_of(0), page1 = page_of(1);
-    int32_t page = page_of(2);
-    locate(0, page0);
-    locate(1, page1);
+    int32_t pages[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) pages[k] = page_of(k);
+    int32_t page = page_of(4);
+#pragma unroll
+    for (int k = 0; k < 4; k++) locate(k, pages[k]);
     __syncthreads();
-    rows.fetch(a, tk.at[0], lane);
+    Rows other = rows;
+    other.fetch(a, tk.at[0], lane);
+    if (kAhead == 2) rows.fetch(a, tk.at[1], lane);
     Query<NG, T> q[1];
     q[0].load(a, a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head, quad);
 
@@ -95,20 +101,21 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
 #pragma unroll
     for (int v = 0; v < VD; v++) vw[v] = min(16 * v + col, a.c.W - 1);
 
-    rows.store(a, lds.rows[0], tk, 0, wave, lane);
-    locate(2, page);
-    page = page_of(3);
-    rows.fetch(a, tk.at[1], lane);
+    other.store(a, lds.rows[0], tk, 0, wave, lane);
+    if (kAhead == 2)
+      other.fetch(a, tk.at[2], lane);
+    else
+      rows.fetch(a, tk.at[1], lane);
 
-    // Stage i is computed with while the rows of the next are written to LDS, those of the one
-    // after are on their way and that one's successor is located: one barrier a stage. (Past the
-    // last stage the last token's page is read.)
-    for (int i = 0; i < stages; i++) {
+    // Stage i is computed with while the rows of the next are written to LDS, those after are on their
+    // way and those of one more are located: one barrier a stage. (Past the last stage the last
+    // token's page is read.)
+    const auto take = [&](int i, Rows& next) {
       __syncthreads();
-      rows.store(a, lds.rows[(i + 1) & 1], tk, i + 1, wave, lane);
-      locate(i + 3, page);
-      page = page_of(i + 4);
-      rows.fetch(a, tk.at[(i + 2) & 3], lane);
+      next.store(a, lds.rows[(i + 1) & 1], tk, i + 1, wave, lane);
+      locate(i + 4, page);
+      page = page_of(i + 5);
+      next.fetch(a, tk.at[(i + 1 + kAhead) & 3], lane);
       const typename Rows::Lds& now = lds.rows[i & 1];
 
       const int t = begin + i * tokens + kTile * static_cast<int>(turn);
@@ -169,6 +176,10 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 4 ? 2 : 4) void attend_rows(At
           pair(std::integral_constant<int, 3>{});
         }
       }
+    };
+    for (int i = 0; i < stages; i += kAhead) {
+      take(i, rows);
+      if (kAhead == 2 && i + 1 < stages) take(i + 1, other);
     }
     __syncthreads();  // the rows have been read
   }
