@@ -1,6 +1,6 @@
 // Attention over a paged cache held in 4 bits: the calls, how their work is dealt out, and the join
-// of contexts that were split (attend.hpp has the mathematics, attend_few.hip and attend_many.hip the
-// kernels).
+// of contexts that were split (attend.hpp has the mathematics, attend_few.hip and attend_many.hip
+// the kernels).
 #include "attend.hpp"
 
 namespace evs {
@@ -8,12 +8,14 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 
-// Rows of a row tile that was split, joined: workgroups for each row tile that there may be and head,
-// which take the tile's rows in turn. A workgroup's threads are dealt a dword of elements each and, as
-// many times over as there are parts for, the parts in turn; the rest of them takes further rows.
+// Rows of a row tile that was split, joined: workgroups for each row tile that there may be and
+// head, which take the tile's rows in turn. A workgroup's threads are dealt a dword of elements
+// each and, as many times over as there are parts for, the parts in turn; the rest of them takes
+// further rows.
 //
-// A launch of its own (about 6 us): joined by the last of a tile's workgroups to end instead, a decode
-// step took 113 us for 86, with parts that pass the caches, and 417 with fences of the GPU's scope.
+// A launch of its own (about 6 us): joined by the last of a tile's workgroups to end instead, a
+// decode step took 113 us for 86, with parts that pass the caches, and 417 with fences of the GPU's
+// scope.
 template <bool kMany, typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a) {
   __shared__ float s_v[kJoinThreads][8 + 1];
@@ -46,7 +48,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a) {
   const uint32_t w = threadIdx.x & (lanes - 1), turn = (threadIdx.x >> a.join_bits) & (turns - 1);
   const uint32_t mine = threadIdx.x >> (a.join_bits + turn_bits);
   const uint32_t wr = min(w, static_cast<uint32_t>(a.c.W) - 1);
-  const uint32_t held = min(1 << dealt.tile_bits, sq.rows - static_cast<int>(tile << dealt.tile_bits));  // rows of it
+  const int row0 = static_cast<int>(tile << dealt.tile_bits);
+  const uint32_t held = min(1 << dealt.tile_bits, sq.rows - row0);  // rows of it
   for (uint32_t r0 = blockIdx.y * rows; r0 < held; r0 += gridDim.y * rows) {
     const uint32_t r = r0 + mine;
     const int row = static_cast<int>(min(r, held - 1));
@@ -84,7 +87,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] += s_v[t][j] * f;
     }
-    finish<T>(a, sq, static_cast<int>((tile << dealt.tile_bits) + r), head, w, v, top, total);
+    finish<T>(a, sq, row0 + static_cast<int>(r), head, w, v, top, total);
   }
 }
 
@@ -159,9 +162,11 @@ Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d
     const int64_t shares = tiles * least(max_len / kMinShare + 1, few_at_once(d));
     r.held = 1;
     for (int64_t n = 2; side_by_side && n <= kFewWaves; n++)
-      if (heads % n == 0 && shares * (heads / n) >= few_at_once(d)) r.held = static_cast<uint32_t>(n);
+      if (heads % n == 0 && shares * (heads / n) >= few_at_once(d))
+        r.held = static_cast<uint32_t>(n);
     r.few.tile_bits = 4;
-    deal_tiles(r.few, r.few_bytes, tiles, most, most * seqs, least(rows, kFewTile), heads / r.held, heads, d,
+    deal_tiles(r.few, r.few_bytes, tiles, most, most * seqs, least(rows, kFewTile),
+               heads / r.held, heads, d,
                max_len, few_at_once(d));
   }
   if (rows > kFewRows) {

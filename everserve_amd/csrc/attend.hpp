@@ -9,11 +9,11 @@
 //
 // Products are MFMA tiles of bf16 with f32 sums: a code times its scale is exact in bf16, so the
 // scores' products are exact for bf16 queries; f16 queries go in as the sum of two bf16 (11 bits of
-// mantissa fit in 8 + 8). The weights exp(s - m) are rounded to bf16 for bf16 outputs (at most half a
-// step, 2^-8 of a weight, of either sign; their sum is taken before that) and are the sum of two
-// bf16 for f16 ones. The scaled MFMA, which would take K's codes and scales as they lie in the cache,
-// is not used for the scores: with queries as sums of e4m3 terms its sums were off by 2^-13 to
-// 2^-17 of the products' magnitudes, where these are off by 2^-24.
+// mantissa fit in 8 + 8). The weights exp(s - m) are rounded to bf16 for bf16 outputs (at most half
+// a step, 2^-8 of a weight, of either sign; their sum is taken before that) and are the sum of two
+// bf16 for f16 ones. The scaled MFMA, which would take K's codes and scales as they lie in the
+// cache, is not used for the scores: with queries as sums of e4m3 terms its sums were off by 2^-13
+// to 2^-17 of the products' magnitudes, where these are off by 2^-24.
 //
 // Both products are computed transposed, so that no value changes lanes between them: the scores
 // leave a lane with four tokens of one query row, and those weights are its part of the second
@@ -29,14 +29,11 @@ constexpr int kManyWaves = 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Sequences with at most kFewRows query rows a KV head go to attend_few in tiles of 16, others to
-// attend_many in tiles of 128, of 64 for head sizes above 128 (their sums take twice the registers).
+// attend_many in tiles of 128, of 64 for head sizes above 128 (their sums take twice the
+// registers).
 constexpr int kFewRows = 64;
 constexpr int kFewTile = 16;
 constexpr int many_tile(int64_t head_dim) { return head_dim > 128 ? 64 : 128; }
-
-// Tokens of a stage: what a workgroup takes at once.
-inline uint32_t few_stage(uint32_t turns) { return 32 * turns; }
-constexpr uint32_t many_stage(int64_t head_dim) { return head_dim > 128 ? 32 : 64; }
 
 // How one kernel's work is dealt out (see Share below and `deal`).
 struct Dealt {
@@ -45,9 +42,9 @@ struct Dealt {
   uint32_t tile_bits;   // log2 of a tile's rows
   int32_t rows;         // of them that are ever used
   float* part;  // [workgroups, 2, heads, rows, d + 2]: a part's sums, running maximum and total
-  // Which shares a split tile is in, for the join. few: [seqs, tiles a sequence may have], the first
-  // and how many (tiles of 16 rows are many, but few of a sequence); many: [workgroups], of the share
-  // with the tile's start, the sequence, the tile and how many, below 2 if there is none.
+  // Which shares a split tile is in, for the join. few: [seqs, tiles a sequence may have], the
+  // first and how many (tiles of 16 rows are many, but few of a sequence); many: [workgroups], of
+  // the share with the tile's start, the sequence, the tile and how many, below 2 if there is none.
   uint4* tiles_in;
   int64_t in;    // entries of it
   FastDiv most;  // tiles that a sequence may have
@@ -138,10 +135,10 @@ __device__ __forceinline__ uint32_t stages_of(const Sequence& q, uint32_t tokens
   return q.len <= 0 ? 1 : (q.len + tokens - 1) / tokens;
 }
 
-// A workgroup's share of the work. All row tiles' stages, sequence by sequence and tile by tile, are
-// one line, cut into equal shares: a workgroup may have the end of a tile, some whole tiles and the
-// start of another. Each finds its share by itself from the lengths, so nothing is planned ahead of
-// the launch. Without splits the line is of whole tiles, one a share.
+// A workgroup's share of the work. All row tiles' stages, sequence by sequence and tile by tile,
+// are one line, cut into equal shares: a workgroup may have the end of a tile, some whole tiles and
+// the start of another. Each finds its share by itself from the lengths, so nothing is planned
+// ahead of the launch. Without splits the line is of whole tiles, one a share.
 //
 // A tile costs its workgroup a start (its queries, its first pages and rows) beside its stages: on
 // the line it has kStart places more, ahead of them.
@@ -161,8 +158,8 @@ constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 8 to 11 us beside ot
 constexpr uint32_t kMinShare = 512;
 
 // Without splits, in the kernel for many rows: row tile `at` from the sequence with the longest
-// context on, and in a sequence from the last one on, which see the most tokens. Workgroups start in
-// this order, so that the last to start have the least to do. For at most as many sequences as
+// context on, and in a sequence from the last one on, which see the most tokens. Workgroups start
+// in this order, so that the last to start have the least to do. For at most as many sequences as
 // threads.
 __device__ __forceinline__ bool longest_first(const AttendArgs& a, uint32_t at, Share& r) {
   __shared__ int32_t s_len[64 * kManyWaves];
@@ -324,14 +321,14 @@ __device__ __forceinline__ int lane_now() {
   return lane;
 }
 
-// The kernel's arguments, read afresh, for the same reason: what a part's start and end need of them is
-// not to take the stages' scalar registers.
+// The kernel's arguments, read afresh, for the same reason: what a part's start and end need of
+// them is not to take the stages' scalar registers.
 __device__ __forceinline__ AttendArgs args_now() {
   uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
   asm volatile("" : "+s"(p));
   AttendArgs a;
-  __builtin_memcpy(&a, (const void*)reinterpret_cast<const __attribute__((address_space(4))) char*>(p),
-                   sizeof(a));
+  typedef const __attribute__((address_space(4))) char* Constant;
+  __builtin_memcpy(&a, (const void*)reinterpret_cast<Constant>(p), sizeof(a));
   return a;
 }
 
@@ -365,10 +362,10 @@ __device__ __forceinline__ float across_rows_sum(float v) {
 }
 
 // ---------------------------------------------------------------- scores
-// Which dword of a half-row's codes product i of the scores takes from quarter `quad` of the lanes: any
-// order will do that is the same for K and the queries. Where the groups are a multiple of four, a
-// quarter has a group's four dwords (one wide read, one scale) for four products; of two groups,
-// half of one for two products; else product i is group i.
+// Which dword of a half-row's codes product i of the scores takes from quarter `quad` of the lanes:
+// any order will do that is the same for K and the queries. Where the groups are a multiple of
+// four, a quarter has a group's four dwords (one wide read, one scale) for four products; of two
+// groups, half of one for two products; else product i is group i.
 template <int NG>
 struct Order {
   static constexpr int kRun = NG % 4 == 0 ? 4 : NG == 2 ? 2 : 1;  // dwords read at once
@@ -407,14 +404,14 @@ struct Query {
   }
 };
 
-// Token t's place among the rows of its 16: a lane's four tokens lie four rows apart, so that the four
-// quarters of a wave read different banks.
+// Token t's place among the rows of its 16: a lane's four tokens lie four rows apart, so that the
+// four quarters of a wave read different banks.
 __device__ __forceinline__ uint32_t place_of(uint32_t t) {
   return (t & ~15u) | ((t & 3) << 2) | ((t >> 2) & 3);
 }
 
-// The scores of 32 tokens, whose codes and scales lie in LDS from row `at` on, with 16 rows' queries,
-// kTiles times over.
+// The scores of 32 tokens, whose codes and scales lie in LDS from row `at` on, with 16 rows'
+// queries, kTiles times over.
 template <int NG, int kTiles, typename T, typename Lds>
 __device__ __forceinline__ void scores(const Lds& lds, int at, int lane, int W,
                                        const Query<NG, T> (&q)[kTiles], f32x4 (&acc)[2][kTiles]) {
@@ -452,8 +449,8 @@ __device__ __forceinline__ void scores(const Lds& lds, int at, int lane, int W,
   }
 }
 
-// A lane's part of the values of 32 tokens from row `at` of LDS on: dword `w` of the codes of tokens
-// 4 quad + r and 16 + 4 quad + r, and their scales' bytes, four to a dword.
+// A lane's part of the values of 32 tokens from row `at` of LDS on: dword `w` of the codes of
+// tokens 4 quad + r and 16 + 4 quad + r, and their scales' bytes, four to a dword.
 struct Values {
   uint32_t codes[8];
   uint32_t scales[2];
@@ -464,7 +461,8 @@ struct Values {
     for (int k = 0; k < 8; k++) codes[k] = lds.codes[1][at + 16 * (k >> 2) + 4 * (k & 3) + quad][w];
 #pragma unroll
     for (int g = 0; g < 2; g++)
-      scales[g] = *reinterpret_cast<const uint32_t*>(&lds.scales[1][w >> 2][at + 16 * g + 4 * quad]);
+      scales[g] =
+          *reinterpret_cast<const uint32_t*>(&lds.scales[1][w >> 2][at + 16 * g + 4 * quad]);
   }
 
   __device__ __forceinline__ void to_f32(float (&scale)[8]) const {
@@ -483,10 +481,9 @@ __device__ __forceinline__ T load_global(uint64_t p) {
 
 // ---------------------------------------------------------------- the cache's rows, through LDS
 // A workgroup's waves together fetch the K and V rows of a stage: kPairs (token, head)
-// pairs a wave, token by token (heads that lie side by side in memory are read side by side), each row as
-// 16-byte chunks and its scale dwords, into registers a stage ahead of their use, then into LDS.
-// There the rows of a head follow one another, and the scale
-// bytes of a group of its tokens.
+// pairs a wave, token by token (heads that lie side by side in memory are read side by side), each
+// row as 16-byte chunks and its scale dwords, into registers a stage ahead of their use, then into
+// LDS. There the rows of a head follow one another, and the scale bytes of a group of its tokens.
 
 //
 // kWhole: the codes are whole chunks (the dwords of a half-row's codes are a multiple of four).
@@ -508,8 +505,8 @@ struct Stage {
     uint32_t nan[4][kWaves];  // the V rows that a wave fetched may hold a group without a number
   };
 
-  // A chunk's token in the stage (8 bits), the dword of it in the cache from the token's first head on
-  // (10 bits: see `deal` on heads that lie side by side) and its dword in LDS (13 bits).
+  // A chunk's token in the stage (8 bits), the dword of it in the cache from the token's first head
+  // on (10 bits: see `deal` on heads that lie side by side) and its dword in LDS (13 bits).
   uint32_t chunk[kLoads];
   uint32_t last;  // the same of the lane's scales, with their row in LDS
   u32x4 codes[2][kLoads];
@@ -524,8 +521,8 @@ struct Stage {
   static __device__ __forceinline__ uint32_t to_of(uint32_t x) { return x >> 18; }
 
   // The stage has `tokens` tokens of `held.d` heads.
-  __device__ __forceinline__ void place(const AttendArgs& a, int wave, int lane, const FastDiv& held,
-                                        uint32_t tokens) {
+  __device__ __forceinline__ void place(const AttendArgs& a, int wave, int lane,
+                                        const FastDiv& held, uint32_t tokens) {
     const uint32_t head_dwords = held.d > 1 ? static_cast<uint32_t>(a.c.sh) >> 2 : 0;
     uint32_t token, h;
 #pragma unroll
@@ -608,9 +605,9 @@ struct Stage {
     if (lane == 0) t.nan[stage & 3][wave] = any;
   }
 
-  // The page of the thread's token of a stage, read a stage before its address is needed. (No branch
-  // stands around this load or those of `fetch`, or the compiler loses count of the loads under way
-  // and waits for all of them.)
+  // The page of the thread's token of a stage, read a stage before its address is needed. (No
+  // branch stands around this load or those of `fetch`, or the compiler loses count of the loads
+  // under way and waits for all of them.)
   static __device__ __forceinline__ int32_t page_of(const AttendArgs& a, const int32_t* table,
                                                     uint32_t t, uint32_t stop) {
     return table[a.c.div_bs.div(min(t, stop - 1))];
@@ -648,7 +645,8 @@ struct Running {
 // The scores of tokens that a row does not see, and of those that are none, masked: `ahead` is the
 // number of tokens from this lane's first of the 32 up to the row's last, `ok` has a bit a token.
 template <int kTiles>
-__device__ __forceinline__ void mask(float (&s)[kTiles][8], const int (&ahead)[kTiles], uint32_t ok) {
+__device__ __forceinline__ void mask(float (&s)[kTiles][8], const int (&ahead)[kTiles],
+                                     uint32_t ok) {
 #pragma unroll
   for (int k = 0; k < 8; k++) {
     const int at = 16 * (k >> 2) + (k & 3);
@@ -669,8 +667,8 @@ __device__ __forceinline__ bool sees_nan(const Lds& lds, int at, int grp, int ah
   return hit;
 }
 
-// Whether eight new scores of each of this lane's rows (masked ones -infinity) take some row's maximum
-// too far past its reference: then all sums so far must be multiplied by `fade`.
+// Whether eight new scores of each of this lane's rows (masked ones -infinity) take some row's
+// maximum too far past its reference: then all sums so far must be multiplied by `fade`.
 template <int kTiles>
 __device__ __forceinline__ bool grow(const float (&s)[kTiles][8], float scale_log2,
                                      Running (&r)[kTiles], float (&fade)[kTiles]) {
@@ -732,7 +730,8 @@ __device__ __forceinline__ void value_pair(const uint32_t (&x)[8], const float (
 }
 
 // ---------------------------------------------------------------- results
-// One dword's eight elements of an output row, from the sums, their reference and the weights' total.
+// One dword's eight elements of an output row, from the sums, their reference and the weights'
+// total.
 template <typename T>
 __device__ __forceinline__ void finish(const AttendArgs& a, const Sequence& sq, int row,
                                        uint32_t head, int w, const float (&v)[8], float top,

@@ -7,9 +7,9 @@ namespace {
 
 constexpr int kTile = 32;  // tokens a wave takes at once
 
-// One workgroup: a share of the stages of tiles of 16 query rows, for a group of KV heads whose rows lie side by
-// side. A stage is 32 tokens of every wave's head; waves with one head take a stage's tokens in
-// turns of 32 and join their results in LDS.
+// One workgroup: a share of the stages of tiles of 16 query rows, for a group of KV heads whose
+// rows lie side by side. A stage is 32 tokens of every wave's head; waves with one head take a
+// stage's tokens in turns of 32 and join their results in LDS.
 template <int NG, bool kWhole, typename T>
 __global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(AttendArgs a) {
   constexpr int kTerms = QueryTerms<T>::n;
@@ -44,210 +44,213 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(At
   Sequence sq = sequence_of_all(a, share.seq);
 
   while (true) {
-  const int lane = lane_now();
-  const int col = lane & 15, quad = lane >> 4;
-  const Part part = next_part<false>(args_now(), sq, share, tokens);
-  if (part.none) return;
-  if (part.slot == 1 && group == 0 && threadIdx.x == 0) {
-    const AttendArgs b = args_now();
-    if (b.few.split) describe<false>(b, share, owner, part);
-  }
-  // this lane's query row, and the tokens that it sees: those up to `sees`
-  uint32_t qi, qg;
-  a.shared.divmod(min(part.row0 + col, part.last_row), qi, qg);
-  const int past = sq.len - sq.nq;
-  const int sees = past + static_cast<int>(qi);
-  // tokens that all of the rows see
-  const int begin = part.begin, stop = part.stop;
-  const int all_see = min(stop, past + static_cast<int>(a.shared.div(part.row0)) + 1);
-  const int stages = stop > begin ? (stop - begin + tokens - 1) / tokens : 0;
-  const int32_t* table = a.tables + static_cast<int64_t>(share.seq) * a.table_stride;
-
-  f32x4 o[VD][8];
-#pragma unroll
-  for (int v = 0; v < VD; v++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[v][j] = f32x4{0, 0, 0, 0};
-  Running run[1];
-
-  if (stages > 0) {
-    Rows rows;
-    rows.place(a, wave, lane, a.held, tokens);
-    const int tid = 64 * wave + lane;
-    // (without a sign: past the last stage it may pass 2^31)
-    const auto token_of = [&](int stage) {
-      return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * tokens + tid);
-    };
-    const auto page_of = [&](int stage) { return Rows::page_of(a, table, token_of(stage), stop); };
-    const auto locate = [&](int stage, int32_t page) {
-      if (64 * wave < tokens)
-        Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, tokens);
-    };
-    int32_t pages[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) pages[k] = page_of(k);
-    int32_t page = page_of(4);
-#pragma unroll
-    for (int k = 0; k < 4; k++) locate(k, pages[k]);
-    __syncthreads();
-    Rows other = rows;
-    other.fetch(a, tk.at[0], lane);
-    if (kAhead == 2) rows.fetch(a, tk.at[1], lane);
-    Query<NG, T> q[1];
-    q[0].load(a, a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head, quad);
-
-    const uint32_t row = h * tokens + kTile * turn;  // this wave's first row of a stage
-    int vw[VD];
-#pragma unroll
-    for (int v = 0; v < VD; v++) vw[v] = min(16 * v + col, a.c.W - 1);
-
-    other.store(a, lds.rows[0], tk, 0, wave, lane);
-    if (kAhead == 2)
-      other.fetch(a, tk.at[2], lane);
-    else
-      rows.fetch(a, tk.at[1], lane);
-
-    // Stage i is computed with while the rows of the next are written to LDS, those after are on their
-    // way and those of one more are located: one barrier a stage. (Past the last stage the last
-    // token's page is read.)
-    const auto take = [&](int i, Rows& next) {
-      __syncthreads();
-      next.store(a, lds.rows[(i + 1) & 1], tk, i + 1, wave, lane);
-      locate(i + 4, page);
-      page = page_of(i + 5);
-      next.fetch(a, tk.at[(i + 1 + kAhead) & 3], lane);
-      const typename Rows::Lds& now = lds.rows[i & 1];
-
-      const int t = begin + i * tokens + kTile * static_cast<int>(turn);
-      if (t < stop) {
-        f32x4 acc[2][1];
-        scores<NG, 1, T>(now, row, lane, a.c.W, q, acc);
-        float s[1][8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][0][k & 3];
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][turn]);
-        const bool whole = t + kTile <= all_see && ok == 0xFFFFFFFFu;
-        bool nan = false;
-        if (!whole) {
-          const int ahead[1] = {sees - t - 4 * quad};
-          mask<1>(s, ahead, ok >> (4 * quad));
-          nan = __builtin_amdgcn_ballot_w64(
-                    tk.nan[i & 3][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
-        }
-        float fade[1];
-        if (grow<1>(s, a.scale_log2, run, fade)) {
-#pragma unroll
-          for (int v = 0; v < VD; v++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[v][j] *= fade[0];
-        }
-        u32x4 p[kTerms];
-        weights<kTerms>(s[0], a.scale_log2, run[0], p);
-#pragma unroll
-        for (int v = 0; v < VD; v++) {
-          Values x;
-          x.load(now, row, quad, vw[v]);
-          float sc[8];
-          x.to_f32(sc);
-          if (nan) {
-            // no number must reach the rows that do not see it: it is added by hand to the others
-#pragma unroll
-            for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
-            if (sees_nan(now, row, min(quad + 4 * v, a.c.NG - 1), sees - t, ok)) {
-#pragma unroll
-              for (int j = 0; j < 8; j++) o[v][j] += __builtin_nanf("");
-            }
-          }
-          const auto pair = [&](auto c_) {
-            constexpr int c = decltype(c_)::value;
-            bf16x8 even, odd;
-            value_pair<c>(x.codes, sc, even, odd);
-#pragma unroll
-            for (int n = 0; n < kTerms; n++) {
-              const bf16x8 pf = __builtin_bit_cast(bf16x8, p[n]);
-              o[v][2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pf, o[v][2 * c], 0, 0, 0);
-              o[v][2 * c + 1] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pf, o[v][2 * c + 1], 0, 0, 0);
-            }
-          };
-          pair(std::integral_constant<int, 0>{});
-          pair(std::integral_constant<int, 1>{});
-          pair(std::integral_constant<int, 2>{});
-          pair(std::integral_constant<int, 3>{});
-        }
-      }
-    };
-    for (int i = 0; i < stages; i += kAhead) {
-      take(i, rows);
-      if (kAhead == 2 && i + 1 < stages) take(i + 1, other);
+    const int lane = lane_now();
+    const int col = lane & 15, quad = lane >> 4;
+    const Part part = next_part<false>(args_now(), sq, share, tokens);
+    if (part.none) return;
+    if (part.slot == 1 && group == 0 && threadIdx.x == 0) {
+      const AttendArgs b = args_now();
+      if (b.few.split) describe<false>(b, share, owner, part);
     }
-    __syncthreads();  // the rows have been read
-  }
-  run[0].l = across_rows_sum(run[0].l);
+    // this lane's query row, and the tokens that it sees: those up to `sees`
+    uint32_t qi, qg;
+    a.shared.divmod(min(part.row0 + col, part.last_row), qi, qg);
+    const int past = sq.len - sq.nq;
+    const int sees = past + static_cast<int>(qi);
+    // tokens that all of the rows see
+    const int begin = part.begin, stop = part.stop;
+    const int all_see = min(stop, past + static_cast<int>(a.shared.div(part.row0)) + 1);
+    const int stages = stop > begin ? (stop - begin + tokens - 1) / tokens : 0;
+    const int32_t* table = a.tables + static_cast<int64_t>(share.seq) * a.table_stride;
 
-  {
-  const AttendArgs b = args_now();
-  const uint32_t held = b.held.d;
-  const int lane = lane_now();
-  const int col = lane & 15, quad = lane >> 4;
-  // Element 8 (4 quad + r) + j of row `col` is o[v][j][r].
-  const auto put = [&](uint32_t at, int r, int w, const float (&x)[8], float top, float total) {
-    if (part.whole)
-      finish<T>(b, sq, part.row0 + r, at, w, x, top, total);
-    else
-      keep(b, part_row(b, b.few, owner, part.slot, at, r), w, x, top, total);
-  };
-  if (b.turns == 1) {
-    if (part.row0 + col <= part.last_row) {
-#pragma unroll
-      for (int v = 0; v < VD; v++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int w = 16 * v + 4 * quad + r;
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[j] = o[v][j][r];
-          if (w < b.c.W) put(head, col, w, x, run[0].m, run[0].l);
-        }
-    }
-  } else {
+    f32x4 o[VD][8];
 #pragma unroll
     for (int v = 0; v < VD; v++)
 #pragma unroll
-      for (int r = 0; r < 4; r++)
+      for (int j = 0; j < 8; j++) o[v][j] = f32x4{0, 0, 0, 0};
+    Running run[1];
+
+    if (stages > 0) {
+      Rows rows;
+      rows.place(a, wave, lane, a.held, tokens);
+      const int tid = 64 * wave + lane;
+      // (without a sign: past the last stage it may pass 2^31)
+      const auto token_of = [&](int stage) {
+        return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * tokens + tid);
+      };
+      const auto page_of = [&](int stage) {
+        return Rows::page_of(a, table, token_of(stage), stop);
+      };
+      const auto locate = [&](int stage, int32_t page) {
+        if (64 * wave < tokens)
+          Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, tokens);
+      };
+      int32_t pages[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          lds.joined.o[wave][col][128 * v + 8 * (4 * quad + r) + j] = o[v][j][r];
-    if (quad == 0) {
-      lds.joined.m[wave][col] = run[0].m;
-      lds.joined.l[wave][col] = run[0].l;
-    }
-    __syncthreads();
-    const int W = b.c.W;
-    for (uint32_t x = threadIdx.x; x < kFewTile * held * W; x += blockDim.x) {
-      const int rh = x / W, w = x - rh * W;
-      uint32_t r_, hh;
-      b.held.divmod(rh, r_, hh);
-      const int r = r_;
-      if (part.row0 + r > part.last_row) break;  // rows ascend
-      float top = -INFINITY;
-      for (uint32_t k = hh; k < held * b.turns; k += held) top = fmaxf(top, lds.joined.m[k][r]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      float total = 0, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      for (uint32_t k = hh; k < held * b.turns; k += held) {
-        const float f = __builtin_amdgcn_exp2f(lds.joined.m[k][r] - ref);
-        total += f * lds.joined.l[k][r];
+      for (int k = 0; k < 4; k++) pages[k] = page_of(k);
+      int32_t page = page_of(4);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] += f * lds.joined.o[k][r][8 * w + j];
+      for (int k = 0; k < 4; k++) locate(k, pages[k]);
+      __syncthreads();
+      Rows other = rows;
+      other.fetch(a, tk.at[0], lane);
+      if (kAhead == 2) rows.fetch(a, tk.at[1], lane);
+      Query<NG, T> q[1];
+      q[0].load(a, a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head, quad);
+
+      const uint32_t row = h * tokens + kTile * turn;  // this wave's first row of a stage
+      int vw[VD];
+#pragma unroll
+      for (int v = 0; v < VD; v++) vw[v] = min(16 * v + col, a.c.W - 1);
+
+      other.store(a, lds.rows[0], tk, 0, wave, lane);
+      if (kAhead == 2)
+        other.fetch(a, tk.at[2], lane);
+      else
+        rows.fetch(a, tk.at[1], lane);
+
+      // Stage i is computed with while the rows of the next are written to LDS, those after are on
+      // their way and those of one more are located: one barrier a stage. (Past the last stage the
+      // last token's page is read.)
+      const auto take = [&](int i, Rows& next) {
+        __syncthreads();
+        next.store(a, lds.rows[(i + 1) & 1], tk, i + 1, wave, lane);
+        locate(i + 4, page);
+        page = page_of(i + 5);
+        next.fetch(a, tk.at[(i + 1 + kAhead) & 3], lane);
+        const typename Rows::Lds& now = lds.rows[i & 1];
+
+        const int t = begin + i * tokens + kTile * static_cast<int>(turn);
+        if (t < stop) {
+          f32x4 acc[2][1];
+          scores<NG, 1, T>(now, row, lane, a.c.W, q, acc);
+          float s[1][8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][0][k & 3];
+          const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][turn]);
+          const bool whole = t + kTile <= all_see && ok == 0xFFFFFFFFu;
+          bool nan = false;
+          if (!whole) {
+            const int ahead[1] = {sees - t - 4 * quad};
+            mask<1>(s, ahead, ok >> (4 * quad));
+            nan = __builtin_amdgcn_ballot_w64(
+                      tk.nan[i & 3][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
+          }
+          float fade[1];
+          if (grow<1>(s, a.scale_log2, run, fade)) {
+#pragma unroll
+            for (int v = 0; v < VD; v++)
+#pragma unroll
+              for (int j = 0; j < 8; j++) o[v][j] *= fade[0];
+          }
+          u32x4 p[kTerms];
+          weights<kTerms>(s[0], a.scale_log2, run[0], p);
+#pragma unroll
+          for (int v = 0; v < VD; v++) {
+            Values x;
+            x.load(now, row, quad, vw[v]);
+            float sc[8];
+            x.to_f32(sc);
+            if (nan) {
+              // no number must reach the rows that do not see it: it is added by hand to the others
+#pragma unroll
+              for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
+              if (sees_nan(now, row, min(quad + 4 * v, a.c.NG - 1), sees - t, ok)) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[v][j] += __builtin_nanf("");
+              }
+            }
+            const auto pair = [&](auto c_) {
+              constexpr int c = decltype(c_)::value;
+              bf16x8 even, odd;
+              value_pair<c>(x.codes, sc, even, odd);
+#pragma unroll
+              for (int n = 0; n < kTerms; n++) {
+                const bf16x8 pf = __builtin_bit_cast(bf16x8, p[n]);
+                o[v][2 * c] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, pf, o[v][2 * c], 0, 0, 0);
+                o[v][2 * c + 1] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, pf, o[v][2 * c + 1], 0, 0, 0);
+              }
+            };
+            pair(std::integral_constant<int, 0>{});
+            pair(std::integral_constant<int, 1>{});
+            pair(std::integral_constant<int, 2>{});
+            pair(std::integral_constant<int, 3>{});
+          }
+        }
+      };
+      for (int i = 0; i < stages; i += kAhead) {
+        take(i, rows);
+        if (kAhead == 2 && i + 1 < stages) take(i + 1, other);
       }
-      put(group * held + hh, r, w, v, top, total);
+      __syncthreads();  // the rows have been read
     }
-  }
-  }
-  if (share.count == 0) return;
-  next_tile<false>(args_now(), part, share, sq);
-  if (share.count == 0) return;
-  __syncthreads();  // LDS is free
+    run[0].l = across_rows_sum(run[0].l);
+
+    {
+    const AttendArgs b = args_now();
+    const uint32_t held = b.held.d;
+    const int lane = lane_now();
+    const int col = lane & 15, quad = lane >> 4;
+    // Element 8 (4 quad + r) + j of row `col` is o[v][j][r].
+    const auto put = [&](uint32_t at, int r, int w, const float (&x)[8], float top, float total) {
+      if (part.whole)
+        finish<T>(b, sq, part.row0 + r, at, w, x, top, total);
+      else
+        keep(b, part_row(b, b.few, owner, part.slot, at, r), w, x, top, total);
+    };
+    if (b.turns == 1) {
+      if (part.row0 + col <= part.last_row) {
+#pragma unroll
+        for (int v = 0; v < VD; v++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int w = 16 * v + 4 * quad + r;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = o[v][j][r];
+            if (w < b.c.W) put(head, col, w, x, run[0].m, run[0].l);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VD; v++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            lds.joined.o[wave][col][128 * v + 8 * (4 * quad + r) + j] = o[v][j][r];
+      if (quad == 0) {
+        lds.joined.m[wave][col] = run[0].m;
+        lds.joined.l[wave][col] = run[0].l;
+      }
+      __syncthreads();
+      const int W = b.c.W;
+      for (uint32_t x = threadIdx.x; x < kFewTile * held * W; x += blockDim.x) {
+        const int rh = x / W, w = x - rh * W;
+        uint32_t r_, hh;
+        b.held.divmod(rh, r_, hh);
+        const int r = r_;
+        if (part.row0 + r > part.last_row) break;  // rows ascend
+        float top = -INFINITY;
+        for (uint32_t k = hh; k < held * b.turns; k += held) top = fmaxf(top, lds.joined.m[k][r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float total = 0, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (uint32_t k = hh; k < held * b.turns; k += held) {
+          const float f = __builtin_amdgcn_exp2f(lds.joined.m[k][r] - ref);
+          total += f * lds.joined.l[k][r];
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] += f * lds.joined.o[k][r][8 * w + j];
+        }
+        put(group * held + hh, r, w, v, top, total);
+      }
+    }
+    }
+    if (share.count == 0) return;
+    next_tile<false>(args_now(), part, share, sq);
+    if (share.count == 0) return;
+    __syncthreads();  // LDS is free
   }
 }
 

@@ -7,10 +7,11 @@ namespace {
 
 constexpr int kTile = 32;     // tokens taken at once
 
-// One workgroup: a share of the stages of tiles of 128 query rows (64 where NG > 4) of one KV head, a
-// quarter of them a wave, which all take every token of a stage. Every wave turns K's codes into
-// operands for itself; V's, which take twice the instructions, are turned into operands once for the
-// four waves, a quarter by each, a stage ahead, and kept in LDS in the order in which lanes read them.
+// One workgroup: a share of the stages of tiles of 128 query rows (64 where NG > 4) of one KV head,
+// a quarter of them a wave, which all take every token of a stage. Every wave turns K's codes into
+// operands for itself; V's, which take twice the instructions, are turned into operands once for
+// the four waves, a quarter by each, a stage ahead, and kept in LDS in the order in which lanes
+// read them.
 template <int NG, bool kWhole, typename T>
 __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a) {
   constexpr int kTerms = QueryTerms<T>::n;
@@ -46,237 +47,239 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
   Sequence sq = sequence_of_all(a, share.seq);
 
   while (true) {
-  const int lane = lane_now();
-  const int col = lane & 15, quad = lane >> 4;
-  const Part part = next_part<true>(a, sq, share, kTokens);
-  if (part.none) return;
-  if (part.slot == 1 && !part.whole && head == 0 && threadIdx.x == 0)
-    describe<true>(a, share, owner, part);
-  const int past = sq.len - sq.nq;
-  const int row0 = part.row0, last_row = part.last_row, begin = part.begin, stop = part.stop;
-  const int stages = stop > begin ? (stop - begin + kTokens - 1) / kTokens : 0;
+    const int lane = lane_now();
+    const int col = lane & 15, quad = lane >> 4;
+    const Part part = next_part<true>(a, sq, share, kTokens);
+    if (part.none) return;
+    if (part.slot == 1 && !part.whole && head == 0 && threadIdx.x == 0)
+      describe<true>(a, share, owner, part);
+    const int past = sq.len - sq.nq;
+    const int row0 = part.row0, last_row = part.last_row, begin = part.begin, stop = part.stop;
+    const int stages = stop > begin ? (stop - begin + kTokens - 1) / kTokens : 0;
 
-  // this wave's rows, and the tokens that some and all of them see
-  const int wave0 = row0 + 16 * kRowTiles * wave;
-  const bool any_row = wave0 <= last_row;
-  const int wave_last = min(wave0 + 16 * kRowTiles - 1, last_row);
-  const int wave_stop =
-      any_row ? min(stop, past + static_cast<int>(a.shared.div(wave_last)) + 1) : 0;
-  const int all_see =
-      any_row ? min(stop, past + static_cast<int>(a.shared.div(wave0)) + 1) : 0;
-  int sees[kRowTiles];
-  const char* qp[kRowTiles];
+    // this wave's rows, and the tokens that some and all of them see
+    const int wave0 = row0 + 16 * kRowTiles * wave;
+    const bool any_row = wave0 <= last_row;
+    const int wave_last = min(wave0 + 16 * kRowTiles - 1, last_row);
+    const int wave_stop =
+        any_row ? min(stop, past + static_cast<int>(a.shared.div(wave_last)) + 1) : 0;
+    const int all_see =
+        any_row ? min(stop, past + static_cast<int>(a.shared.div(wave0)) + 1) : 0;
+    int sees[kRowTiles];
+    const char* qp[kRowTiles];
 #pragma unroll
-  for (int n = 0; n < kRowTiles; n++) {
-    uint32_t qi, qg;
-    a.shared.divmod(min(wave0 + 16 * n + col, last_row), qi, qg);
-    sees[n] = past + static_cast<int>(qi);
-    qp[n] = a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head;
-  }
+    for (int n = 0; n < kRowTiles; n++) {
+      uint32_t qi, qg;
+      a.shared.divmod(min(wave0 + 16 * n + col, last_row), qi, qg);
+      sees[n] = past + static_cast<int>(qi);
+      qp[n] = a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head;
+    }
 
-  const int32_t* table = a.tables + static_cast<int64_t>(share.seq) * a.table_stride;
+    const int32_t* table = a.tables + static_cast<int64_t>(share.seq) * a.table_stride;
 
-  f32x4 o[kRowTiles][VD][8];
+    f32x4 o[kRowTiles][VD][8];
 #pragma unroll
-  for (int n = 0; n < kRowTiles; n++)
+    for (int n = 0; n < kRowTiles; n++)
 #pragma unroll
-    for (int v = 0; v < VD; v++)
+      for (int v = 0; v < VD; v++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) o[n][v][j] = f32x4{0, 0, 0, 0};
-  Running run[kRowTiles];
+        for (int j = 0; j < 8; j++) o[n][v][j] = f32x4{0, 0, 0, 0};
+    Running run[kRowTiles];
 
-  if (stages > 0) {
-    Rows rows;
-    rows.place(a, wave, lane, a.one, kTokens);
-    const int tid = 64 * wave + lane;
-    // (without a sign: past the last stage it may pass 2^31)
-    const auto token_of = [&](int stage) {
-      return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * kTokens + tid);
-    };
-    const auto page_of = [&](int stage) { return Rows::page_of(a, table, token_of(stage), stop); };
-    const auto locate = [&](int stage, int32_t page) {
-      if (64 * wave < kTokens)
-        Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, kTokens);
-    };
-    int32_t pages[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) pages[k] = page_of(k);
-    int32_t page = page_of(4);
-#pragma unroll
-    for (int k = 0; k < 4; k++) locate(k, pages[k]);
-    __syncthreads();
-    Rows second = rows;
-    rows.fetch(a, tk.at[0], lane);
-    second.fetch(a, tk.at[1], lane);
-    Query<NG, T> q[kRowTiles];
-#pragma unroll
-    for (int n = 0; n < kRowTiles; n++) q[n].load(a, qp[n], quad);
-
-    // this wave's quarter of V's operands: half of the elements of a dword of 32 tokens
-    const int vsub = VD == 1 ? wave >> 1 : 0, vv = VD == 1 ? 0 : wave >> 1;
-    const int vw = min(16 * vv + col, a.c.W - 1);
-    const auto any_nan = [&](int stage) {
-      return __builtin_amdgcn_ballot_w64(tk.nan[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
-    };
-    const auto convert = [&](int stage, int at, bool nan) {
-      Values x;
-      x.load(lds[at], kTile * vsub, quad, vw);
-      float sc[8];
-      x.to_f32(sc);
-      if (nan) {  // no number is added by hand below, to the rows that see it
-#pragma unroll
-        for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
-      }
-      auto* to = &s_value[stage & 1][vsub][vv];
-      const auto pair = [&](auto c_) {
-        constexpr int c = decltype(c_)::value;
-        bf16x8 even, odd;
-        value_pair<c>(x.codes, sc, even, odd);
-        (*to)[2 * c][lane] = even;
-        (*to)[2 * c + 1][lane] = odd;
+    if (stages > 0) {
+      Rows rows;
+      rows.place(a, wave, lane, a.one, kTokens);
+      const int tid = 64 * wave + lane;
+      // (without a sign: past the last stage it may pass 2^31)
+      const auto token_of = [&](int stage) {
+        return static_cast<uint32_t>(begin) + static_cast<uint32_t>(stage * kTokens + tid);
       };
-      if (wave & 1) {
-        pair(std::integral_constant<int, 2>{});
-        pair(std::integral_constant<int, 3>{});
-      } else {
-        pair(std::integral_constant<int, 0>{});
-        pair(std::integral_constant<int, 1>{});
-      }
-    };
-    rows.store(a, lds[0], tk, 0, wave, lane);
-    second.store(a, lds[1], tk, 1, wave, lane);
-    rows.fetch(a, tk.at[2], lane);
-    __syncthreads();
-    convert(0, 0, any_nan(0));
-
-    // Stage i is computed with while the values of the next are converted, the rows of the one after
-    // are written to LDS and those of a third are on their way: one barrier a stage. (Past the last
-    // stage the last token's page is read.)
-    int now = 0, ahead1 = 1, ahead2 = 2;  // where the stages' rows lie in LDS
-    bool nan = false, nan_next = any_nan(0);
-    f32x4 first[2][kRowTiles];
-    scores<NG, kRowTiles, T>(lds[0], 0, lane, a.c.W, q, first);
-    for (int i = 0; i < stages; i++) {
+      const auto page_of = [&](int stage) {
+        return Rows::page_of(a, table, token_of(stage), stop);
+      };
+      const auto locate = [&](int stage, int32_t page) {
+        if (64 * wave < kTokens)
+          Rows::locate(a, tk, stage, base, token_of(stage), stop, page, tid, kTokens);
+      };
+      int32_t pages[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) pages[k] = page_of(k);
+      int32_t page = page_of(4);
+#pragma unroll
+      for (int k = 0; k < 4; k++) locate(k, pages[k]);
       __syncthreads();
-      rows.store(a, lds[ahead2], tk, i + 2, wave, lane);
-      locate(i + 4, page);
-      page = page_of(i + 5);
-      rows.fetch(a, tk.at[(i + 3) & 3], lane);
-      nan = nan_next;
-      nan_next = any_nan(i + 1);
-      convert(i + 1, ahead1, nan_next);
-      const int t0 = begin + i * kTokens;
+      Rows second = rows;
+      rows.fetch(a, tk.at[0], lane);
+      second.fetch(a, tk.at[1], lane);
+      Query<NG, T> q[kRowTiles];
+#pragma unroll
+      for (int n = 0; n < kRowTiles; n++) q[n].load(a, qp[n], quad);
 
-      // 32 tokens, whose scores are in `acc`; those of the next 32 go to `after`, beside the products
-      // with the values: their codes are converted while the matrix cores have these.
-      const auto take = [&](int sub, f32x4 (&acc)[2][kRowTiles], int rows_after, int at_after,
-                            f32x4 (&after)[2][kRowTiles]) {
-        const int t = t0 + kTile * sub;
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][sub]);
-        float s[kRowTiles][8];
+      // this wave's quarter of V's operands: half of the elements of a dword of 32 tokens
+      const int vsub = VD == 1 ? wave >> 1 : 0, vv = VD == 1 ? 0 : wave >> 1;
+      const int vw = min(16 * vv + col, a.c.W - 1);
+      const auto any_nan = [&](int stage) {
+        return __builtin_amdgcn_ballot_w64(tk.nan[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
+      };
+      const auto convert = [&](int stage, int at, bool nan) {
+        Values x;
+        x.load(lds[at], kTile * vsub, quad, vw);
+        float sc[8];
+        x.to_f32(sc);
+        if (nan) {  // no number is added by hand below, to the rows that see it
 #pragma unroll
-        for (int n = 0; n < kRowTiles; n++)
-#pragma unroll
-          for (int k = 0; k < 8; k++) s[n][k] = acc[k >> 2][n][k & 3];
-        if (t + kTile > all_see || ok != 0xFFFFFFFFu) {
-          int ahead[kRowTiles];
-#pragma unroll
-          for (int n = 0; n < kRowTiles; n++) ahead[n] = sees[n] - t - 4 * quad;
-          mask<kRowTiles>(s, ahead, ok >> (4 * quad));
+          for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
         }
-        float fade[kRowTiles];
-        if (grow<kRowTiles>(s, a.scale_log2, run, fade)) {
+        auto* to = &s_value[stage & 1][vsub][vv];
+        const auto pair = [&](auto c_) {
+          constexpr int c = decltype(c_)::value;
+          bf16x8 even, odd;
+          value_pair<c>(x.codes, sc, even, odd);
+          (*to)[2 * c][lane] = even;
+          (*to)[2 * c + 1][lane] = odd;
+        };
+        if (wave & 1) {
+          pair(std::integral_constant<int, 2>{});
+          pair(std::integral_constant<int, 3>{});
+        } else {
+          pair(std::integral_constant<int, 0>{});
+          pair(std::integral_constant<int, 1>{});
+        }
+      };
+      rows.store(a, lds[0], tk, 0, wave, lane);
+      second.store(a, lds[1], tk, 1, wave, lane);
+      rows.fetch(a, tk.at[2], lane);
+      __syncthreads();
+      convert(0, 0, any_nan(0));
+
+      // Stage i is computed with while the values of the next are converted, the rows of the one
+      // after are written to LDS and those of a third are on their way: one barrier a stage. (Past
+      // the last stage the last token's page is read.)
+      int now = 0, ahead1 = 1, ahead2 = 2;  // where the stages' rows lie in LDS
+      bool nan = false, nan_next = any_nan(0);
+      f32x4 first[2][kRowTiles];
+      scores<NG, kRowTiles, T>(lds[0], 0, lane, a.c.W, q, first);
+      for (int i = 0; i < stages; i++) {
+        __syncthreads();
+        rows.store(a, lds[ahead2], tk, i + 2, wave, lane);
+        locate(i + 4, page);
+        page = page_of(i + 5);
+        rows.fetch(a, tk.at[(i + 3) & 3], lane);
+        nan = nan_next;
+        nan_next = any_nan(i + 1);
+        convert(i + 1, ahead1, nan_next);
+        const int t0 = begin + i * kTokens;
+
+        // 32 tokens, whose scores are in `acc`; those of the next 32 go to `after`, beside the
+        // products with the values: their codes are converted while the matrix cores have these.
+        const auto take = [&](int sub, f32x4 (&acc)[2][kRowTiles], int rows_after, int at_after,
+                              f32x4 (&after)[2][kRowTiles]) {
+          const int t = t0 + kTile * sub;
+          const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][sub]);
+          float s[kRowTiles][8];
 #pragma unroll
           for (int n = 0; n < kRowTiles; n++)
 #pragma unroll
-            for (int v = 0; v < VD; v++)
+            for (int k = 0; k < 8; k++) s[n][k] = acc[k >> 2][n][k & 3];
+          if (t + kTile > all_see || ok != 0xFFFFFFFFu) {
+            int ahead[kRowTiles];
 #pragma unroll
-              for (int j = 0; j < 8; j++) o[n][v][j] *= fade[n];
-        }
-        if (nan) {
+            for (int n = 0; n < kRowTiles; n++) ahead[n] = sees[n] - t - 4 * quad;
+            mask<kRowTiles>(s, ahead, ok >> (4 * quad));
+          }
+          float fade[kRowTiles];
+          if (grow<kRowTiles>(s, a.scale_log2, run, fade)) {
+#pragma unroll
+            for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+              for (int v = 0; v < VD; v++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[n][v][j] *= fade[n];
+          }
+          if (nan) {
+#pragma unroll
+            for (int v = 0; v < VD; v++) {
+              const int grp = min(quad + 4 * v, a.c.NG - 1);
+#pragma unroll
+              for (int n = 0; n < kRowTiles; n++)
+                if (sees_nan(lds[now], kTile * sub, grp, sees[n] - t, ok)) {
+#pragma unroll
+                  for (int j = 0; j < 8; j++) o[n][v][j] += __builtin_nanf("");
+                }
+            }
+          }
+          u32x4 p[kRowTiles][kTerms];
 #pragma unroll
           for (int v = 0; v < VD; v++) {
-            const int grp = min(quad + 4 * v, a.c.NG - 1);
+            // all reads are under way before the weights are computed and the first product waits
+            bf16x8 x[8];
 #pragma unroll
-            for (int n = 0; n < kRowTiles; n++)
-              if (sees_nan(lds[now], kTile * sub, grp, sees[n] - t, ok)) {
+            for (int j = 0; j < 8; j++) x[j] = s_value[i & 1][sub][v][j][lane];
+            __builtin_amdgcn_sched_barrier(0);
+            if (v == 0) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) o[n][v][j] += __builtin_nanf("");
-              }
+              for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+              for (int n = 0; n < kRowTiles; n++)
+#pragma unroll
+                for (int m = 0; m < kTerms; m++)
+                  o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      x[j], __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
+          }
+          scores<NG, kRowTiles, T>(lds[rows_after], at_after, lane, a.c.W, q, after);
+          __builtin_amdgcn_s_setprio(0);
+        };
+        if (t0 < wave_stop) {
+          if (kSubs == 1) {
+            take(0, first, ahead1, 0, first);
+          } else {
+            f32x4 second_half[2][kRowTiles];
+            take(0, first, now, kTile, second_half);
+            if (t0 + kTile < wave_stop)
+              take(1, second_half, ahead1, 0, first);
           }
         }
-        u32x4 p[kRowTiles][kTerms];
-#pragma unroll
-        for (int v = 0; v < VD; v++) {
-          // all reads are under way before the weights are computed and the first product waits
-          bf16x8 x[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[j] = s_value[i & 1][sub][v][j][lane];
-          __builtin_amdgcn_sched_barrier(0);
-          if (v == 0) {
-#pragma unroll
-            for (int n = 0; n < kRowTiles; n++) weights<kTerms>(s[n], a.scale_log2, run[n], p[n]);
-          }
-          __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-          for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int n = 0; n < kRowTiles; n++)
-#pragma unroll
-              for (int m = 0; m < kTerms; m++)
-                o[n][v][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    x[j], __builtin_bit_cast(bf16x8, p[n][m]), o[n][v][j], 0, 0, 0);
-        }
-        scores<NG, kRowTiles, T>(lds[rows_after], at_after, lane, a.c.W, q, after);
-        __builtin_amdgcn_s_setprio(0);
-      };
-      if (t0 < wave_stop) {
-        if (kSubs == 1) {
-          take(0, first, ahead1, 0, first);
-        } else {
-          f32x4 second_half[2][kRowTiles];
-          take(0, first, now, kTile, second_half);
-          if (t0 + kTile < wave_stop)
-            take(1, second_half, ahead1, 0, first);
-        }
+        const int free = now;
+        now = ahead1;
+        ahead1 = ahead2;
+        ahead2 = free;
       }
-      const int free = now;
-      now = ahead1;
-      ahead1 = ahead2;
-      ahead2 = free;
+      __syncthreads();  // the rows and values have been read
     }
-    __syncthreads();  // the rows and values have been read
-  }
 
-  {
-  const int lane = lane_now();
-  const int col = lane & 15, quad = lane >> 4;
-  // Element 8 (4 quad + r) + j of row `col` of a tile is o[n][v][j][r].
+    {
+    const int lane = lane_now();
+    const int col = lane & 15, quad = lane >> 4;
+    // Element 8 (4 quad + r) + j of row `col` of a tile is o[n][v][j][r].
 #pragma unroll
-  for (int n = 0; n < kRowTiles; n++) {
-    const float l = across_rows_sum(run[n].l);
-    const int row = wave0 + 16 * n + col;
-    if (row > last_row) continue;
+    for (int n = 0; n < kRowTiles; n++) {
+      const float l = across_rows_sum(run[n].l);
+      const int row = wave0 + 16 * n + col;
+      if (row > last_row) continue;
 #pragma unroll
-    for (int v = 0; v < VD; v++)
+      for (int v = 0; v < VD; v++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int w = 16 * v + 4 * quad + r;
-        float x[8];
+        for (int r = 0; r < 4; r++) {
+          const int w = 16 * v + 4 * quad + r;
+          float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = o[n][v][j][r];
-        if (w >= a.c.W) continue;
-        if (part.whole)
-          finish<T>(a, sq, row, head, w, x, run[n].m, l);
-        else
-          keep(a, part_row(a, a.many, owner, part.slot, head, row - row0), w, x, run[n].m, l);
-      }
-  }
-  }
-  if (share.count == 0) return;
-  next_tile<true>(a, part, share, sq);
-  if (share.count == 0) return;
-  __syncthreads();  // LDS is free
+          for (int j = 0; j < 8; j++) x[j] = o[n][v][j][r];
+          if (w >= a.c.W) continue;
+          if (part.whole)
+            finish<T>(a, sq, row, head, w, x, run[n].m, l);
+          else
+            keep(a, part_row(a, a.many, owner, part.slot, head, row - row0), w, x, run[n].m, l);
+        }
+    }
+    }
+    if (share.count == 0) return;
+    next_tile<true>(a, part, share, sq);
+    if (share.count == 0) return;
+    __syncthreads();  // LDS is free
   }
 }
 

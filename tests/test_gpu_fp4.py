@@ -351,3 +351,118 @@ def test_queries_that_want_a_gradient_are_refused(ext):
         cache.attend(q.detach(), tables.cuda(), lens, out=torch.zeros(1, 1, 64, device="cuda"))
     with pytest.raises(RuntimeError, match="int32"):
         cache.attend(q.detach(), tables.cuda().long(), lens)
+
+
+# ---------------------------------------------------------------- how the work is dealt out
+@pytest.mark.parametrize("heads", [1, 2, 3, 5, 6, 7, 8, 10, 12])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_heads_that_lie_side_by_side_are_taken_together(ext, heads, layout):
+    # enough sequences that a workgroup takes as many heads as it can; lengths about a stage's and a
+    # share's ends
+    lens = [0, 1, 31, 32, 33, 255, 256, 257, 511, 513, 640, 7] * 10
+    attend_case(layout, 16, heads, 1, 32, "bf16", lens, [1] * len(lens), seed=heads, max_len=4096)
+
+
+@pytest.mark.parametrize("d,dtype", [(24, "f16"), (96, "bf16"), (128, "f16"), (192, "bf16"),
+                                     (256, "f16")])
+def test_tiles_in_several_shares_of_unlike_sequences(ext, d, dtype):
+    # shares that end in a tile, in the next one and at a tile's start
+    lens = [5000, 3, 0, 1300, 1024, 2048, 1, 700, 3333]
+    attend_case("kv_first", 16, 2, 2, d, dtype, lens, [1] * len(lens), seed=d)
+    attend_case("combined", 24, 1, 3, d, dtype, lens, [7, 3, 2, 11, 1, 5, 1, 16, 4], seed=d)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "bf16"), (72, "f16"), (128, "bf16"), (200, "f16")])
+def test_long_chunks_are_split_too(ext, d, dtype):
+    attend_case("kv_first", 16, 1, 5, d, dtype, [2100, 1500, 90, 4000], [40, 130, 90, 14], seed=d)
+
+
+@pytest.mark.parametrize("seqs", [257, 513, 1100])
+def test_more_sequences_than_a_workgroup_has_threads(ext, seqs):
+    lens = [(37 * i) % 90 for i in range(seqs)]
+    lens[seqs // 2], lens[-1] = 1500, 1100
+    attend_case("combined", 16, 1, 2, 16, "bf16", lens, [1] * seqs, seed=seqs)
+    news = [1 + (i % 3) * 20 for i in range(seqs)]
+    attend_case("kv_first", 16, 1, 2, 16, "bf16", lens, news, seed=seqs)
+    attend_case("kv_first", 16, 1, 2, 16, "bf16", [min(n, 80) for n in lens], news, seed=seqs)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("news,shared", [(3, 4), (16, 1), (100, 2), (33, 5)])
+@pytest.mark.parametrize("back", [0, 1, 2])
+def test_no_number_in_a_masked_place(ext, d, news, shared, back):
+    """A token whose V holds a group without a number, at the last places of a chunk: the rows before
+    it are as without it, in the same products' tile."""
+    n = 200
+    cache, tables = filled("kv_first", 16, 1, d, [n, n], 6)
+    at = n - 1 - back
+    x = torch.ones(1, 1, d, device="cuda")
+    x[0, 0, d - 10] = math.inf
+    slot = tables[0, at // 16].long().reshape(1).cuda() * 16 + at % 16
+    q = torch.randn(2 * news, shared, d, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    how = dict(q_starts=torch.tensor([0, news, 2 * news]).int().cuda(), max_q=news)
+    lens = torch.tensor([n, n], device="cuda").int()
+    ones = torch.ones_like(x)
+    cache.write(slot, ones, ones)
+    want = cache.attend(q, tables.cuda(), lens, **how)
+    cache.write(slot, ones, x)
+    out = cache.attend(q, tables.cuda(), lens, **how)
+    hit = news - 1 - back  # the first query that sees the token
+    bad = torch.isnan(out)
+    rows = slice(max(hit, 0), news)
+    group = slice((d - 10) // 32 * 32, min(d, (d - 10) // 32 * 32 + 32))
+    assert bad[rows, :, group].all()
+    bad[rows, :, group] = False
+    assert not bad.any()
+    same = torch.ones_like(bad)
+    same[rows, :, group] = False
+    assert torch.equal(out[same], want[same])
+    # and a K without a number: the rows that see it are none, the others as they were
+    cache.write(slot, x, ones)
+    out = cache.attend(q, tables.cuda(), lens, **how)
+    assert torch.isnan(out[rows]).all() and torch.equal(out[:rows.start], want[:rows.start])
+    assert torch.equal(out[news:], want[news:])
+
+
+def test_padding_queries_that_no_sequence_names_are_left_alone(ext):
+    cache, tables = filled("kv_first", 16, 1, 64, [300, 40], 6)
+    q = torch.randn(90, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    lens = torch.tensor([300, 40]).int().cuda()
+    for starts in ([0, 1, 31], [3, 60, 62], [10, 10, 50]):
+        out = torch.full_like(q, 7.0)
+        cache.attend(q, tables.cuda(), lens, q_starts=torch.tensor(starts).int().cuda(), max_q=60,
+                     out=out)
+        assert torch.all(out[:starts[0]] == 7) and torch.all(out[starts[2]:] == 7)
+        part = q[starts[0]:starts[2]].contiguous()
+        own = torch.tensor([s - starts[0] for s in starts]).int().cuda()
+        want = cache.attend(part, tables.cuda(), lens, q_starts=own, max_q=60)
+        assert torch.equal(out[starts[0]:starts[2]], want)
+
+
+def test_a_captured_batch_replays_with_other_lengths(ext):
+    """The shares are found on the device: a graph holds for any lengths."""
+    lens0 = [3000, 40, 700, 0]
+    cache, tables = filled("combined", 16, 2, 64, [4000, 900, 900, 900], 8)
+    dev = tables.cuda()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(90, 8, 64, device="cuda", generator=g).bfloat16()
+    lens = torch.tensor(lens0, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 1, 2, 80, 81], dtype=torch.int32, device="cuda")
+
+    def step():
+        return cache.attend(q, dev, lens, q_starts=starts, max_q=80, return_lse=True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for new, at in (([3000, 40, 700, 0], [0, 1, 2, 80, 81]), ([4000, 900, 80, 3], [0, 9, 10, 11, 90]),
+                    ([1, 2, 3, 4], [0, 1, 2, 3, 4]), ([0, 0, 900, 900], [0, 80, 81, 82, 90])):
+        lens.copy_(torch.tensor(new, dtype=torch.int32))
+        starts.copy_(torch.tensor(at, dtype=torch.int32))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        n = at[-1]
+        assert torch.equal(got[0][:n], want[0][:n]) and torch.equal(got[1][:n], want[1][:n])
