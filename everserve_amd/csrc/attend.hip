@@ -115,10 +115,14 @@ constexpr int64_t kCus = 256;
 int64_t few_at_once(int64_t d) { return (d > 64 ? 1 : 2) * kCus; }
 constexpr int64_t kManyAtOnce = 2 * kCus;
 
+constexpr int64_t kFewRows[] = {64, 128};
+constexpr int64_t kLittle = 1 << 18;  // tokens of all sequences and KV heads
+
 // How a call's work is dealt out, from its counts alone (the lengths are on the device).
 struct Deal {
   Dealt few, many;
   uint32_t held;  // KV heads that a workgroup of attend_few takes
+  int64_t few_rows;
   int64_t few_bytes, many_bytes;  // of the parts' workspace
 };
 
@@ -147,14 +151,25 @@ void place_parts(Dealt& r, void* at) {
   r.part = reinterpret_cast<float*>(static_cast<char*>(at) + r.in * 16);
 }
 
+// The most query rows a KV head of a sequence that attend_few takes. Up to 64, it wins throughout
+// (32 heads on 8 of 128, us, it for attend_many: 4 sequences of 4 to 8 Ki tokens 50 for 70; 64 of 1
+// to 2 Ki with 48 rows 87 for 131, with 64 level). From there to 128 it wins while there is little
+// to do, where tiles of 128 rows leave most CUs idle: 4 sequences of 4 to 8 Ki with 128 rows 63 for
+// 80, 16 of 1 to 2 Ki 65 for 78; but 24 of them 86 for 81, 32 107 for 85, 16 of 4 to 8 Ki 173 for
+// 115.
+int64_t few_rows(int64_t seqs, int64_t heads, int64_t max_len) {
+  return max_len > 0 && seqs * heads > kLittle / max_len ? kFewRows[0] : kFewRows[1];
+}
+
 Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d, int64_t max_q,
-          int64_t max_len, bool side_by_side) {
+          int64_t max_len, int64_t few_rows, bool side_by_side) {
   Deal r{};
   const auto least = [](int64_t x, int64_t y) { return x < y ? x : y; };
   const int64_t rows = max_q * shared;
+  r.few_rows = few_rows;
   // row tiles: a sequence's rows, rounded up
-  if (shared <= kFewRows) {
-    const int64_t most = (least(rows, kFewRows) + kFewTile - 1) / kFewTile;
+  if (shared <= r.few_rows) {
+    const int64_t most = (least(rows, r.few_rows) + kFewTile - 1) / kFewTile;
     const int64_t tiles = least(most * seqs, tokens * shared / kFewTile + seqs);
     // The most heads, up to the waves, that leave shares for all workgroups: heads that lie side by
     // side share memory lines (8 of 128: 5.4 TB/s, in fours 4.4 and in twos 3.2), but the more of
@@ -166,10 +181,9 @@ Deal deal(int64_t seqs, int64_t tokens, int64_t shared, int64_t heads, int64_t d
         r.held = static_cast<uint32_t>(n);
     r.few.tile_bits = 4;
     deal_tiles(r.few, r.few_bytes, tiles, most, most * seqs, least(rows, kFewTile),
-               heads / r.held, heads, d,
-               max_len, few_at_once(d));
+               heads / r.held, heads, d, max_len, few_at_once(d));
   }
-  if (rows > kFewRows) {
+  if (rows > r.few_rows) {
     const int64_t tile = many_tile(d);
     const int64_t most = (rows + tile - 1) / tile;
     const int64_t tiles = least(most * seqs, tokens * shared / tile + seqs);
@@ -196,12 +210,15 @@ extern "C" int evs_fp4_attend_workspace(int64_t seqs, int64_t tokens, int64_t q_
               "evs_fp4_attend_workspace: bad count");
   if (seqs == 0 || tokens == 0 || max_q == 0) return EVS_OK;
   if (max_len == 0) max_len = INT64_MAX;
-  for (const bool side_by_side : {false, true}) {
-    const evs::Deal deal = evs::deal(seqs, tokens, q_heads / heads, heads, head_dim,
-                                     max_q < tokens ? max_q : tokens, max_len, side_by_side);
-    const int64_t need = deal.few_bytes + deal.many_bytes;
-    if (need > *bytes) *bytes = need;
-  }
+  // (the call takes max_len up to the tables' room: less may change who takes which rows)
+  for (const int64_t few_rows : evs::kFewRows)
+    for (const bool side_by_side : {false, true}) {
+      const evs::Deal deal =
+          evs::deal(seqs, tokens, q_heads / heads, heads, head_dim,
+                    max_q < tokens ? max_q : tokens, max_len, few_rows, side_by_side);
+      const int64_t need = deal.few_bytes + deal.many_bytes;
+      if (need > *bytes) *bytes = need;
+    }
   return EVS_OK;
 }
 
@@ -263,7 +280,8 @@ extern "C" int evs_fp4_attend(const void* q, const int64_t* q_strides, int type,
   // a workgroup takes several heads where a token's rows of them follow one another
   const bool side_by_side = strides[2] > 0 && strides[2] <= 2 * evs::fp4_row_bytes(head_dim);
   const evs::Deal deal =
-      evs::deal(seqs, tokens, shared, heads, head_dim, max_q, max_len, side_by_side);
+      evs::deal(seqs, tokens, shared, heads, head_dim, max_q, max_len,
+                evs::few_rows(seqs, heads, max_len), side_by_side);
   const int64_t tiles =
       (static_cast<int64_t>(deal.few.workgroups) + deal.many.workgroups) * heads;
   EVS_REQUIRE(tiles < (int64_t{1} << 24), "%s: %lld tiles of query rows: below 2^24", who,
@@ -274,6 +292,7 @@ extern "C" int evs_fp4_attend(const void* q, const int64_t* q_strides, int type,
                                  reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
               "%s: a workspace of %lld bytes on 16, %lld needed", who,
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  a.few_rows = static_cast<int32_t>(deal.few_rows);
   a.few = deal.few;
   a.many = deal.many;
   if (need > 0) {

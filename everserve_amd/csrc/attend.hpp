@@ -28,10 +28,9 @@ constexpr int kFewWaves = 8;   // of a workgroup, at most
 constexpr int kManyWaves = 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Sequences with at most kFewRows query rows a KV head go to attend_few in tiles of 16, others to
-// attend_many in tiles of 128, of 64 for head sizes above 128 (their sums take twice the
-// registers).
-constexpr int kFewRows = 64;
+// Sequences with at most `few_rows` query rows a KV head (the call chooses) go to attend_few in tiles of
+// 16, others to attend_many in tiles of 128, of 64 for head sizes above 128 (their sums take twice
+// the registers).
 constexpr int kFewTile = 16;
 constexpr int many_tile(int64_t head_dim) { return head_dim > 128 ? 64 : 128; }
 
@@ -71,6 +70,7 @@ struct AttendArgs {
   FastDiv groups;      // such groups of heads
   uint32_t join_bits;  // log2 of a joined row's dwords, rounded up
   FastDiv heads;
+  int32_t few_rows;
   Dealt few, many;
 };
 
@@ -127,7 +127,7 @@ __device__ __forceinline__ unsigned long long scalar(unsigned long long v) {
 template <bool kMany>
 __device__ __forceinline__ uint32_t tiles_of(const AttendArgs& a, const Sequence& q) {
   const uint32_t bits = (kMany ? a.many : a.few).tile_bits;
-  return (q.rows > kFewRows) == kMany ? (q.rows + (1u << bits) - 1) >> bits : 0;
+  return (q.rows > a.few_rows) == kMany ? (q.rows + (1u << bits) - 1) >> bits : 0;
 }
 
 // Stages of `tokens` that a row tile takes; an empty context takes one too, that it is answered.
@@ -153,8 +153,10 @@ struct Share {
 template <bool kMany>
 constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 8 to 11 us beside others, a stage 3
 
-// The fewest stages of a share, in tokens: a stage takes about 1 us where nothing else runs, and
-// the join of a split context 5 us.
+// The fewest stages of a share, in tokens; contexts of up to twice as many are not split. With half
+// as many a context of 600 tokens took 13.4 us for 12.3 and 16 sequences of up to 2,000 21.2 for
+// 21.8. With twice as many one of 4,000 took 19.0 for 17.5, and a batch with one long chunk 107 for
+// 99; 4 sequences of 4 to 8 Ki with 128 rows 80 for 100.
 constexpr uint32_t kMinShare = 512;
 
 // Without splits, in the kernel for many rows: row tile `at` from the sequence with the longest

@@ -377,6 +377,15 @@ def test_long_chunks_are_split_too(ext, d, dtype):
     attend_case("kv_first", 16, 1, 5, d, dtype, [2100, 1500, 90, 4000], [40, 130, 90, 14], seed=d)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, "f16"), (128, "bf16"), (192, "bf16")])
+@pytest.mark.parametrize("seqs,max_len", [(5, 0), (300, 0), (300, 1 << 20)])
+def test_65_to_128_query_rows_of_a_head(ext, d, dtype, seqs, max_len):
+    # the rows go to either kernel by how much there is to do, up to the tables' room
+    lens = [1100] + [40 + 7 * (i % 9) for i in range(seqs - 1)]
+    news = [[26, 32, 17, 33, 1][i % 5] for i in range(seqs)]
+    attend_case("blocks_first", 16, 1, 4, d, dtype, lens, news, seed=d, max_len=max_len)
+
+
 @pytest.mark.parametrize("seqs", [257, 513, 1100])
 def test_more_sequences_than_a_workgroup_has_threads(ext, seqs):
     lens = [(37 * i) % 90 for i in range(seqs)]
