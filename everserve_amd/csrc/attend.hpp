@@ -28,9 +28,9 @@ constexpr int kFewWaves = 8;   // of a workgroup, at most
 constexpr int kManyWaves = 4;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Sequences with at most `few_rows` query rows a KV head (the call chooses) go to attend_few in tiles of
-// 16, others to attend_many in tiles of 128, of 64 for head sizes above 128 (their sums take twice
-// the registers).
+// Sequences with at most `few_rows` query rows a KV head (the call chooses) go to attend_few in
+// tiles of 16, others to attend_many in tiles of 128, of 64 for head sizes above 128 (their sums
+// take twice the registers).
 constexpr int kFewTile = 16;
 constexpr int many_tile(int64_t head_dim) { return head_dim > 128 ? 64 : 128; }
 
@@ -151,7 +151,7 @@ struct Share {
   unsigned long long line, size;  // the tile's start on the line, places of a share
 };
 template <bool kMany>
-constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 8 to 11 us beside others, a stage 3
+constexpr uint32_t kStart = kMany ? 2 : 3;  // a start took 2 to 4 times as long as a stage
 
 // The fewest stages of a share, in tokens; contexts of up to twice as many are not split. With half
 // as many a context of 600 tokens took 13.4 us for 12.3 and 16 sequences of up to 2,000 21.2 for
