@@ -13,10 +13,11 @@ constexpr int kJoinThreads = 256;
 // each and, as many times over as there are parts for, the parts in turn; the rest of them takes
 // further rows.
 //
-// A launch of its own, bound by its latency: 4 to 7 us after attend_few (a decode step of 64
-// sequences 4.8), 15 to 19 after attend_many with up to 128 rows of a tile. Joined by the last of a
-// tile's workgroups to end instead, a decode step that took 86 us then took 113 with parts that
-// pass the caches, and 417 with fences of the GPU's scope.
+// A launch of its own. After attend_few it is bound by latency: 4 to 7 us, a decode step of 64
+// sequences 4.8. After attend_many it is bound by the parts' bytes: up to two a workgroup of 128
+// rows, 68 MB for heads of 128, in 15 to 19 us. Joined by the last of a tile's workgroups to end
+// instead, a decode step that took 86 us then took 113 with parts that pass the caches, and 417 with
+// fences of the GPU's scope.
 template <bool kMany, typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_parts(AttendArgs a) {
   __shared__ float s_v[kJoinThreads][8 + 1];
