@@ -473,6 +473,23 @@ struct Values {
   }
 };
 
+// Scales from 2^126 on, and the one of a group without a number: a code times such a scale may be
+// no finite number, which times the weight 0 of a row that does not see the token is NaN. Such
+// groups of V are kept out of the products' operands (tame) and added by hand to the rows that see
+// their token (add_wild).
+constexpr uint32_t kWildByte = 253;
+constexpr float kWildScale = 0x1p126f;  // as scale_of has it
+
+// Eight tokens' codes and scales without the wild ones.
+__device__ __forceinline__ void tame(uint32_t (&codes)[8], float (&scale)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const bool wild = scale[k] >= kWildScale;
+    codes[k] = wild ? 0 : codes[k];
+    scale[k] = wild ? 1.0f : scale[k];
+  }
+}
+
 // A value at a device address that is a multiple of four; an address out of LDS must say so, or the
 // load counts as one that may be of LDS and is waited for with those.
 template <typename T>
@@ -504,7 +521,7 @@ struct Stage {
   struct Tokens {
     uint64_t at[4][kRowsOf];
     uint32_t ok[8][kRowsOf / 32];
-    uint32_t nan[4][kWaves];  // the V rows that a wave fetched may hold a group without a number
+    uint32_t wild[4][kWaves];  // the V rows that a wave fetched may hold a wild group (kWildByte)
   };
 
   // A chunk's token in the stage (8 bits), the dword of it in the cache from the token's first head
@@ -592,19 +609,19 @@ struct Stage {
     const uint32_t row = to_of(y);
     const int kv = lane & kPairs ? 1 : 0;
     const bool ok = (t.ok[stage & 7][token_of(y) >> 5] >> (y & 31)) & 1;
-    bool nan = false;
+    bool wild = false;
 #pragma unroll
     for (int k = 0; k < kScaleDwords; k++) {
       // a token outside the context must be a number, whatever its row holds: its weight is 0
       const uint32_t x = ok ? scale[k] : 0x7F7F7F7Fu;
-      // a byte of ~x is 0 (or a 1 above such a byte)
-      nan |= ((~x - 0x01010101u) & x & 0x80808080u) != 0;
+      // a byte of ~x is below 3 (or a 3 above such a byte)
+      wild |= ((~x - 0x03030303u) & x & 0x80808080u) != 0;
 #pragma unroll
       for (int g = 4 * k; g < NG && g < 4 * k + 4; g++)
         lds.scales[kv][g][row] = static_cast<uint8_t>(x >> (8 * (g & 3)));
     }
-    const bool any = __builtin_amdgcn_ballot_w64(nan && kv) != 0;
-    if (lane == 0) t.nan[stage & 3][wave] = any;
+    const bool any = __builtin_amdgcn_ballot_w64(wild && kv) != 0;
+    if (lane == 0) t.wild[stage & 3][wave] = any;
   }
 
   // The page of the thread's token of a stage, read a stage before its address is needed. (No
@@ -658,17 +675,6 @@ __device__ __forceinline__ void mask(float (&s)[kTiles][8], const int (&ahead)[k
   }
 }
 
-// Whether a row sees a token of the 32 from row `at` of LDS whose V has no number in group `grp`;
-// `ahead` counts from the first of the 32.
-template <typename Lds>
-__device__ __forceinline__ bool sees_nan(const Lds& lds, int at, int grp, int ahead, uint32_t ok) {
-  bool hit = false;
-#pragma unroll 1
-  for (int k = 0; k < 32; k++)
-    hit |= lds.scales[1][grp][at + k] == kScaleNaN && k <= ahead && ((ok >> k) & 1);
-  return hit;
-}
-
 // Whether eight new scores of each of this lane's rows (masked ones -infinity) take some row's
 // maximum too far past its reference: then all sums so far must be multiplied by `fade`.
 template <int kTiles>
@@ -711,6 +717,45 @@ __device__ __forceinline__ void weights(const float (&s)[8], float scale_log2, R
     if (kTerms > 1)
       p[kTerms - 1][k / 2] = pack_bf16(lo - __builtin_bit_cast(float, w << 16),
                                        hi - __builtin_bit_cast(float, w & 0xFFFF0000u));
+  }
+}
+
+// The products of the wild groups of V (kWildByte) among the 32 tokens from row `at` of LDS, whose
+// scores for this lane's row are `s`: the lane's elements of o[j][r] (dword 16 v + 4 quad + r, one
+// group) get them if its row sees the token. `ahead` counts from the first of the 32.
+template <typename Lds>
+__device__ __forceinline__ void add_wild(const Lds& lds, int at, int v, int W, int ahead,
+                                         uint32_t ok, const float (&s)[8], float scale_log2,
+                                         const Running& r, f32x4 (&o)[8]) {
+  const int lane = lane_now();
+  const int quad = lane >> 4, w0 = 16 * v + 4 * quad;
+  Running now = r;  // its shift is not to be shared with the weights', on the way of all stages
+  asm volatile("" : "+v"(now.m));
+  const float shift = now.shift();
+#pragma unroll 1
+  for (int k = 0; k < 32; k++) {
+    // the token's score is with the lanes of quarter k / 4 % 4
+    float mine = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) mine = 4 * (k >> 4) + (k & 3) == i ? s[i] : mine;
+    mine = __shfl(mine, (lane & 15) + 16 * ((k >> 2) & 3));
+    const uint32_t byte = lds.scales[1][min(w0, W - 1) >> 2][at + k];
+    if (byte < kWildByte || k > ahead || !((ok >> k) & 1)) continue;
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(mine, scale_log2, -shift));
+    const float scale = scale_of(byte);
+    const uint32_t* row = lds.codes[1][at + place_of(k)];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t x = row[min(w0 + i, W - 1)];
+      const auto pair = [&](int c, f32x2 value) {
+        o[2 * c][i] += p * value[0];
+        o[2 * c + 1][i] += p * value[1];
+      };
+      pair(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, 0));
+      pair(1, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, 1));
+      pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, 2));
+      pair(3, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x, scale, 3));
+    }
   }
 }
 

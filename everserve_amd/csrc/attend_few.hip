@@ -141,12 +141,12 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(At
           for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][0][k & 3];
           const uint32_t ok = __builtin_amdgcn_readfirstlane(tk.ok[i & 7][turn]);
           const bool whole = t + kTile <= all_see && ok == 0xFFFFFFFFu;
-          bool nan = false;
+          bool wild = false;
           if (!whole) {
             const int ahead[1] = {sees - t - 4 * quad};
             mask<1>(s, ahead, ok >> (4 * quad));
-            nan = __builtin_amdgcn_ballot_w64(
-                      tk.nan[i & 3][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
+            wild = __builtin_amdgcn_ballot_w64(
+                       tk.wild[i & 3][min(lane, static_cast<int>(held * a.turns) - 1)] != 0) != 0;
           }
           float fade[1];
           if (grow<1>(s, a.scale_log2, run, fade)) {
@@ -154,6 +154,11 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(At
             for (int v = 0; v < VD; v++)
 #pragma unroll
               for (int j = 0; j < 8; j++) o[v][j] *= fade[0];
+          }
+          if (wild) {
+#pragma unroll
+            for (int v = 0; v < VD; v++)
+              add_wild(now, row, v, a.c.W, sees - t, ok, s[0], a.scale_log2, run[0], o[v]);
           }
           u32x4 p[kTerms];
           weights<kTerms>(s[0], a.scale_log2, run[0], p);
@@ -163,15 +168,7 @@ __global__ __launch_bounds__(64 * kFewWaves, NG > 2 ? 2 : 4) void attend_rows(At
             x.load(now, row, quad, vw[v]);
             float sc[8];
             x.to_f32(sc);
-            if (nan) {
-              // no number must reach the rows that do not see it: it is added by hand to the others
-#pragma unroll
-              for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
-              if (sees_nan(now, row, min(quad + 4 * v, a.c.NG - 1), sees - t, ok)) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) o[v][j] += __builtin_nanf("");
-              }
-            }
+            if (wild) tame(x.codes, sc);
             const auto pair = [&](auto c_) {
               constexpr int c = decltype(c_)::value;
               bf16x8 even, odd;

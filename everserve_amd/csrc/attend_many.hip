@@ -129,18 +129,15 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
       // this wave's quarter of V's operands: half of the elements of a dword of 32 tokens
       const int vsub = VD == 1 ? wave >> 1 : 0, vv = VD == 1 ? 0 : wave >> 1;
       const int vw = min(16 * vv + col, a.c.W - 1);
-      const auto any_nan = [&](int stage) {
-        return __builtin_amdgcn_ballot_w64(tk.nan[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
+      const auto any_wild = [&](int stage) {
+        return __builtin_amdgcn_ballot_w64(tk.wild[stage & 3][lane & (kManyWaves - 1)] != 0) != 0;
       };
-      const auto convert = [&](int stage, int at, bool nan) {
+      const auto convert = [&](int stage, int at, bool wild) {
         Values x;
         x.load(lds[at], kTile * vsub, quad, vw);
         float sc[8];
         x.to_f32(sc);
-        if (nan) {  // no number is added by hand below, to the rows that see it
-#pragma unroll
-          for (int k = 0; k < 8; k++) sc[k] = sc[k] == INFINITY ? 1.0f : sc[k];
-        }
+        if (__builtin_expect(wild, false)) tame(x.codes, sc);
         auto* to = &s_value[stage & 1][vsub][vv];
         const auto pair = [&](auto c_) {
           constexpr int c = decltype(c_)::value;
@@ -161,13 +158,13 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
       second.store(a, lds[1], tk, 1, wave, lane);
       rows.fetch(a, tk.at[2], lane);
       __syncthreads();
-      convert(0, 0, any_nan(0));
+      convert(0, 0, any_wild(0));
 
       // Stage i is computed with while the values of the next are converted, the rows of the one
       // after are written to LDS and those of a third are on their way: one barrier a stage. (Past
       // the last stage the last token's page is read.)
       int now = 0, ahead1 = 1, ahead2 = 2;  // where the stages' rows lie in LDS
-      bool nan = false, nan_next = any_nan(0);
+      bool wild = false, wild_next = any_wild(0);
       f32x4 first[2][kRowTiles];
       scores<NG, kRowTiles, T>(lds[0], 0, lane, a.c.W, q, first);
       for (int i = 0; i < stages; i++) {
@@ -176,9 +173,9 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
         locate(i + 4, page);
         page = page_of(i + 5);
         rows.fetch(a, tk.at[(i + 3) & 3], lane);
-        nan = nan_next;
-        nan_next = any_nan(i + 1);
-        convert(i + 1, ahead1, nan_next);
+        wild = wild_next;
+        wild_next = any_wild(i + 1);
+        convert(i + 1, ahead1, wild_next);
         const int t0 = begin + i * kTokens;
 
         // 32 tokens, whose scores are in `acc`; those of the next 32 go to `after`, beside the
@@ -207,17 +204,13 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void attend_tiles(AttendArgs a)
 #pragma unroll
                 for (int j = 0; j < 8; j++) o[n][v][j] *= fade[n];
           }
-          if (nan) {
+          if (__builtin_expect(wild, false)) {
 #pragma unroll
-            for (int v = 0; v < VD; v++) {
-              const int grp = min(quad + 4 * v, a.c.NG - 1);
+            for (int v = 0; v < VD; v++)
 #pragma unroll
               for (int n = 0; n < kRowTiles; n++)
-                if (sees_nan(lds[now], kTile * sub, grp, sees[n] - t, ok)) {
-#pragma unroll
-                  for (int j = 0; j < 8; j++) o[n][v][j] += __builtin_nanf("");
-                }
-            }
+                add_wild(lds[now], kTile * sub, v, a.c.W, sees[n] - t, ok, s[n],
+                         a.scale_log2, run[n], o[n][v]);
           }
           u32x4 p[kRowTiles][kTerms];
 #pragma unroll
