@@ -41,6 +41,14 @@ __device__ __forceinline__ int64_t word_offset(const CopyArgs& a, uint32_t w) {
   return off + q * a.stride[a.dims - 1];
 }
 
+// A word of a page. The host has checked every stride and run for it, but the layers' bases are in
+// device memory and may lie on any element, so it claims no alignment (the instructions are those
+// of aligned words).
+template <typename T>
+struct Word {
+  typedef T type __attribute__((aligned(1)));
+};
+
 // The words of all pairs' pages, one after another, dealt to workgroups in tiles: a tile's loads
 // are issued before its first store. A pair with a page the cache does not have, or whose pages
 // are one, moves nothing.
@@ -73,14 +81,15 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages(CopyArgs a) {
         if (s != d && s >= 0 && d >= 0 && s < a.num_blocks && d < a.num_blocks) {
           const int64_t off = word_offset<T>(a, w);
           x[k] = __builtin_nontemporal_load(
-              reinterpret_cast<const T*>(base + s * a.block_bytes + off));
+              reinterpret_cast<const typename Word<T>::type*>(base + s * a.block_bytes + off));
           to[k] = base + d * a.block_bytes + off;
         }
       }
     }
 #pragma unroll
     for (int k = 0; k < kCopyWords; k++)
-      if (to[k] != nullptr) __builtin_nontemporal_store(x[k], reinterpret_cast<T*>(to[k]));
+      if (to[k] != nullptr)
+        __builtin_nontemporal_store(x[k], reinterpret_cast<typename Word<T>::type*>(to[k]));
   }
 }
 

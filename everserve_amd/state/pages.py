@@ -73,6 +73,7 @@ class PageMover:
         self.elem = first.element_size()
         if self.elem not in (1, 2, 4):
             raise ValueError(f"elements of {self.elem} bytes: 1, 2 or 4")
+        # the copy takes any base; the gathers read such caches in aligned words of 16 bytes
         if all(s * self.elem % 16 == 0 for s in self.strides[:4]) and any(
                 t.data_ptr() % 16 for t in layers):
             raise ValueError("caches with strides of whole 16-byte words must start on one")

@@ -279,8 +279,7 @@ int evs_fp4_attend(const void* q, const int64_t* q_strides, int type, void* out,
  * caches addressed as in evs_gather_rows (strides in elements, all positive), num_blocks pages
  * each. `count` (device, int32), if not NULL, cuts the list short. A pair with an id outside
  * [0, num_blocks), or src == dst, moves nothing. Destinations must be distinct and none may be
- * another pair's source. Where every stride and run of a page is a multiple of 16 bytes the layer
- * bases must be too, as for evs_gather_rows. */
+ * another pair's source. The layer bases may lie on any element. */
 int evs_copy_blocks(const int64_t* layer_ptrs, int64_t num_layers, const int32_t* src,
                     const int32_t* dst, int64_t num_pairs, const int32_t* count,
                     int64_t num_blocks, int64_t num_heads, int64_t head_dim, int64_t block_size,
