@@ -28,6 +28,7 @@ import ctypes
 import functools
 import json
 import logging
+import math
 import os
 from dataclasses import dataclass
 from pathlib import Path
@@ -813,7 +814,11 @@ class Kernels:
         ``out`` ([tokens, q_heads, d], written into if given), with ``return_lse`` also the f32
         [tokens, q_heads] logs of the sums of exp(scores). A row that sees nothing is zeros, its
         log -infinity; a page id outside the cache holds nothing. There is no backward pass.
-        Enqueued on the current stream; its workspace comes from torch's allocator."""
+        Enqueued on the current stream; its workspace comes from torch's allocator.
+
+        Rows that no sequence names, and a sequence's past its first ``max_q``, are not written: in
+        a new ``out`` they hold whatever the memory held, unless the call has no sequence or a
+        ``max_q`` of 0 (then all rows see nothing)."""
         import torch
 
         type_ = _row_types().get(q.dtype, 2)
@@ -843,13 +848,17 @@ class Kernels:
             max_q = 1 if q_starts is None else tokens
         if not (cache.is_cuda and block_tables.is_cuda):
             raise RuntimeError("fp4_attend: the cache and the tables must be on the device")
+        idle = seqs == 0 or max_q == 0  # no row is written
         if out is None:
-            out = torch.empty((tokens, q_heads, d), dtype=q.dtype, device=q.device)
+            new = torch.zeros if idle else torch.empty
+            out = new((tokens, q_heads, d), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise RuntimeError("fp4_attend: out must be contiguous and like the queries")
         lse = None
         if return_lse:
             lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
+            if idle:
+                lse.fill_(-math.inf)
         _one_device("fp4_attend", q, cache, block_tables, seq_lens, q_starts, out)
         max_len = max_len or width * block_size
         counts = (seqs, tokens, q_heads, heads, d, max_q, max_len)
