@@ -56,7 +56,7 @@ def main() -> None:
         for c in caches:
             c.write(slots, rows(len(slots), HEADS), rows(len(slots), HEADS))
             c.attend(rows(len(slots), HEADS * SHARED), tables[:4].cuda(), ints(lens),
-                     q_starts=ints(starts), max_q=max(news))
+                     q_starts=ints(starts), max_q=max(news), max_len=max(lens))
         done = lens
 
     # sequences 4 and 5 part from sequence 0: they share its whole pages and copy its last one
@@ -80,7 +80,7 @@ def main() -> None:
         slots = torch.cat([slots_of(s, [lens[s] - 1]) for s in range(6)])
         for c in caches:
             c.write(slots, rows(6, HEADS), rows(6, HEADS))
-            out = c.attend(q, dev, n)
+            out = c.attend(q, dev, n, max_len=max(lens))
     torch.cuda.synchronize()
     print(f"decoded 40 tokens of 6 sequences in {1e3 * (time.perf_counter() - start):.1f} ms, "
           f"{LAYERS} layers")
@@ -89,10 +89,10 @@ def main() -> None:
     kept = [0, 1, 3, 4, 5]
     dev, n = tables[kept].contiguous().cuda(), ints([lens[s] for s in kept])
     counts = ints([-(-lens[s] // PAGE) for s in kept])
-    want = [c.attend(q[:5], dev, n) for c in caches]
+    want = [c.attend(q[:5], dev, n, max_len=max(lens)) for c in caches]
     plan = mover.compact(dev, counts)
     for c, w in zip(caches, want):
-        assert torch.equal(c.attend(q[:5], plan.tables, n), w)
+        assert torch.equal(c.attend(q[:5], plan.tables, n, max_len=max(lens)), w)
     used, moved = plan.sizes.tolist()
     print(f"packed {used} pages to the front by moving {moved}: pages from {used} on are free, "
           f"every answer is as it was")
