@@ -816,6 +816,13 @@ class Kernels:
         log -infinity; a page id outside the cache holds nothing. There is no backward pass.
         Enqueued on the current stream; its workspace comes from torch's allocator.
 
+        Scores, maxima and sums are f32; the weights that multiply V are rounded to bf16 for bf16
+        queries (2^-8 of a weight at most) and to the sum of two bf16 for f16 ones (2^-17).
+
+        How the work is split follows from ``max_len``, or else from the tables' width: give it
+        where tables are much wider than their contexts (four of 600 tokens under tables for
+        131,072: 13 us with it, 35 without).
+
         Rows that no sequence names, and a sequence's past its first ``max_q``, are not written: in
         a new ``out`` they hold whatever the memory held, unless the call has no sequence or a
         ``max_q`` of 0 (then all rows see nothing)."""

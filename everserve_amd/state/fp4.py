@@ -3,7 +3,9 @@
 A half-row (the K or V of one slot and head) is ``head_dim / 2`` bytes of E2M1 codes, one
 power-of-two scale byte for each 32 elements, and zeros up to a multiple of 4 bytes: the MXFP4 of
 the Open Compute microscaling formats, which gfx950's conversions read as it is. 128 elements are 68
-bytes instead of 256.
+bytes instead of 256. The scale that a write chooses is the least power of two that brings the
+group's largest magnitude to 7 or below. That text takes the largest's exponent less 2: the same,
+but where the largest is between 7 and 8 steps of it, which then is cut to 6.
 
 The cache is a uint8 tensor of any of the three layouts with the half-row's bytes in the place of
 the head size, so everything that moves a cache moves it as it stands: the stager, the restore, the
@@ -88,8 +90,9 @@ class Fp4Cache:
     @classmethod
     def empty(cls, num_blocks: int, block_size: int, heads: int, head_dim: int,
               layout: CacheLayout | str = CacheLayout.COMBINED, device="cuda") -> "Fp4Cache":
-        """A new cache, every row of it zeros. ``combined`` keeps a head's page contiguous, which
-        the attention reads fastest."""
+        """A new cache, every row of it zeros. ``combined`` keeps a head's page contiguous; single
+        tokens over many heads are read faster where a token's heads lie side by side, as in the
+        other two (64 sequences of 1 to 8 Ki tokens, 8 heads of 128: 78 us for 91)."""
         import torch
 
         shape = cache_shape(layout, num_blocks, block_size, heads, head_dim)

@@ -257,12 +257,16 @@ int evs_fp4_read_rows(const void* cache, int64_t num_blocks, int64_t block_size,
  *         q_strides: token and head strides in elements;
  *   out   contiguous [tokens, q_heads, head_dim] of `type`, starting on 16 bytes;
  *   lse   contiguous f32 [tokens, q_heads], the natural log of the sum of exp(scores), or NULL.
+ * Scores, maxima and sums are f32. A token's weight exp(s - m) enters its product with V as one bf16
+ * for bf16 queries (off by 2^-8 of itself at most) and as the sum of two for f16 ones (2^-17); lse
+ * is of the weights before that.
  * A row that sees nothing gives zeros, and lse -infinity. A value that is no finite f32 (some codes
  * times 2^126 or 2^127: no write makes them) counts as an infinity; it, and a group without a
  * number, reach the rows that see their token and no others. A table entry outside [0, num_blocks)
  * holds nothing: its tokens are masked. A length is taken up to width * block_size, a sequence's
  * queries up to max_q and `tokens`. Queries that no sequence names are not written. `max_len` (0:
- * width * block_size) is at least the longest length, and only steers how the work is split.
+ * width * block_size) is at least the longest length, and only steers how the work is split: far
+ * above the lengths it leaves most of the GPU idle.
  * `workspace` is device memory of evs_fp4_attend_workspace bytes for the same counts, 16-byte
  * aligned, that no overlapping call uses. The call allocates nothing and may be captured. */
 int evs_fp4_attend_workspace(int64_t seqs, int64_t tokens, int64_t q_heads, int64_t heads,
