@@ -15,7 +15,7 @@ constexpr int kJoinThreads = 256;
 //
 // A launch of its own. After attend_few it is bound by latency: 4 to 7 us, a decode step of 64
 // sequences 4.8. After attend_many it is bound by the parts' bytes: up to two a workgroup of 128
-// rows, 68 MB for heads of 128, in 15 to 19 us. Joined by the last of a tile's workgroups to end
+// rows, 68 MB for heads of 128, in 14 to 19 us. Joined by the last of a tile's workgroups to end
 // instead, a decode step that took 86 us then took 113 with parts that pass the caches, and 417
 // with fences of the GPU's scope.
 template <bool kMany, typename T>

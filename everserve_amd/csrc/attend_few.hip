@@ -12,14 +12,15 @@ constexpr int kTile = 32;  // tokens a wave takes at once
 // stage's tokens in turns of 32 and join their results in LDS.
 //
 // Bound by reading pages at random places. 64 sequences of 1 to 8 Ki tokens, 32 heads on 8 of 128,
-// 322 MB: 75 us, 4.3 TB/s (a loop that only fetches the same rows took 63, 5.1; a large plain copy
+// 322 MB: 76 us, 4.2 TB/s (a loop that only fetches the same rows took 63, 5.1; a large plain copy
 // reaches 4.84 and a plain read 6.3). About 8 us of it are the start, in which three loads wait for
 // each other (a length, page ids, rows). So:
 // - a stage's rows are fetched by all waves together, a token's heads in one run of memory, into
 //   registers, two stages before their use, and pass through LDS with one barrier a stage (fetched
 //   by each wave for its own head: 84 us);
 // - one workgroup a CU with the registers of two, for heads above 64: two leave room for one stage
-//   under way (the decode step above 84 us for 82, with f16 queries 120 for 92);
+//   under way (the call of the decode step above 80 us for 78, with f16 queries 112 for 87; where
+//   a page has a head's rows together, `combined`, 85 for 91 and 118 for 106);
 // - codes become bf16 operands in registers, right before the products; a tile is 16 rows, as wide
 //   as an MFMA, since there are mostly fewer.
 template <int NG, bool kWhole, typename T>

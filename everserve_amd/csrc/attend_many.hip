@@ -16,8 +16,9 @@ constexpr int kTile = 32;  // tokens taken at once
 // Bound by the instructions beside the products: for 32 rows and 32 tokens about 185 vector ones
 // (codes to operands, exponentials, maxima, sums), and with the registers that 128 rows take a SIMD
 // has two waves to fill its matrix unit from, which works 30 % of the time. The last chunks of four
-// prompts (1,024 queries each of 4 to 8 Ki tokens, 32 heads on 8 of 128; 360 GFLOP, 88 MB): 500 us,
-// 720 TFLOP/s, where a large plain bf16 product reaches 1,202. What carries it:
+// prompts (1,024 queries each of 4 to 8 Ki tokens, 32 heads on 8 of 128; 360 GFLOP, 88 MB): 505 us
+// a call, 713 TFLOP/s, where a large plain bf16 product reaches 1,202 (with f16 queries 1.4 times
+// as long). A whole prompt of 8,000 tokens: 1,105 us, 475 TFLOP/s (see stages_of). What carries it:
 // - 128 rows a tile share the conversion of V, and two row tiles of a wave that of K (in tiles of
 //   16 rows, each with its own conversions, the chunks took 811 us, in these 573);
 // - the next 32 tokens' scores are under way while the weights of these are taken, across stages

@@ -66,11 +66,11 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 // nearest, ties to even, by the hardware's conversion.
 //
 // K's group and V's at the same place are one work item: they share the index arithmetic, and both
-// their loads are under way before the first is needed (as two: 56 us for the 44 that 8,192 rows
-// written and 32,768 read take).
+// their loads are under way before the first is needed (a call of 8,192 rows written and one of
+// 32,768 read, 8 heads of 128: 50.8 us together, as two items 66.9).
 //
-// Bound by memory where there are many rows: 8,192 tokens of 8 heads of 128 in 10.9 us, 3.9 TB/s
-// (a large plain copy reaches 4.84). A step's 64 rows are the launch alone.
+// Bound by memory where there are many rows: 8,192 tokens of 8 heads of 128 in 11.0 us, 3.9 TB/s
+// (a large plain copy reaches 4.84). A step's 64 rows are the launch alone (3.2 us).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void write_rows(RowsIo a) {
   const uint32_t u = blockIdx.x * kThreads + threadIdx.x;
@@ -129,7 +129,7 @@ __device__ __forceinline__ T from_f32(float v) {
 
 // One lane turns a dword of K's codes and the one of V's at the same place into eight elements
 // each, so that a wave's stores are whole lines. Bound by them: 32,768 tokens of 8 heads of 128 in
-// bf16 in 32.2 us, 5.3 TB/s.
+// bf16 in 32 us, 5.3 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void read_rows(RowsIo a) {
   const uint32_t unit = blockIdx.x * kThreads + threadIdx.x;

@@ -8,7 +8,8 @@
 //   zeros up to a multiple of 4 bytes.
 // These are the operands of gfx950's scaled conversions, which turn two codes and a scale into two
 // bf16 or f32 values in one full-rate instruction (132 lane-operations per ns and CU measured, as
-// an FMA), exactly: a code times a power of two has two significant bits.
+// an FMA), exactly: a code times a power of two has two significant bits. (Some codes times 2^126
+// or 2^127 are past f32 and bf16, and become infinities; no write makes those scales.)
 #pragma once
 
 #include "common.hpp"
@@ -75,12 +76,9 @@ inline int fp4_cache(const char* who, const void* cache, int64_t num_blocks, int
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __builtin_bit_cast(float, byte << 23);  // 255 gives an exponent that converts to NaN

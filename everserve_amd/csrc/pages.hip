@@ -54,8 +54,8 @@ struct Word {
 // are one, moves nothing.
 //
 // Bound by memory, as a large plain copy is (4.84 TB/s): 64 pages of 64 KiB in each of 32 layers 53
-// us, 5.0 TB/s; the moves of a compaction, 531 MB, 98 us, 5.4. Four words a thread keep enough under
-// way for that.
+// us, 5.0 TB/s; the moves of a compaction, 531 MB, 99 us, 5.4. Four words a thread keep enough
+// under way for that.
 template <typename T>
 __global__ __launch_bounds__(kCopyThreads) void copy_pages(CopyArgs a) {
   char* base = reinterpret_cast<char*>(a.layer_ptrs[blockIdx.y]);
@@ -214,9 +214,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_emit(PlanArgs a) {
 }
 
 // The bitmap and its counts by one workgroup, in LDS; for small tables and caches the whole plan
-// (kWhole). A launch costs about 2 us here and 3 on the host: the plan of 2,304 entries and 2,048
-// pages took 11 us in four launches and takes 6 in this one. Emitting by one workgroup is slower
-// from about 4,096 entries on (13,568 entries and 16,384 pages: 28 us against 13).
+// (kWhole). A launch costs about 2 us here and 3 on the host. In a graph, us a plan:
+//   entries, pages     one launch   two    four
+//    2,368,  2,048         6.8              11.1
+//    4,096,  2,048         7.7              15.3
+//    6,144,  2,048         9.5      7.7     18.3
+//   13,400, 16,384        30.8     11.5     13.9
+//   32,768, 16,384        51       14       20
+// (random tables of 16,384 pages: 2,048 entries 9.7 in one launch, 4,096 13.6, 6,144 10.0 in two).
 constexpr uint32_t kOneWords = 4096;  // 131,072 pages
 constexpr int64_t kOneEntries = 1 << 15;
 constexpr uint32_t kWholeWords = 512;
