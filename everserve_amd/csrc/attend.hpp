@@ -26,7 +26,6 @@ namespace evs {
 
 constexpr int kFewWaves = 8;   // of a workgroup, at most
 constexpr int kManyWaves = 4;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Sequences with at most `few_rows` query rows a KV head (the call chooses) go to attend_few in
 // tiles of 16, others to attend_many in tiles of 128, of 64 for head sizes above 128 (their sums
@@ -107,20 +106,6 @@ __device__ __forceinline__ Sequence sequence_of_all(const AttendArgs& a, uint32_
   r.len = __builtin_amdgcn_readfirstlane(r.len);
   r.rows = __builtin_amdgcn_readfirstlane(r.rows);
   return r;
-}
-
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
-// A value that all lanes have alike, as a scalar.
-__device__ __forceinline__ unsigned long long scalar(unsigned long long v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return static_cast<unsigned long long>(hi) << 32 | lo;
 }
 
 // Row tiles of a sequence in the kernel for many rows, or in that for few.
@@ -319,15 +304,7 @@ __device__ __forceinline__ void next_tile(const AttendArgs& a, const Part& p, Sh
   r.count = 0;
 }
 
-// The lane's number, afresh: what is computed from it is computed in every part, where the compiler
-// would move it ahead of all parts and keep it in registers that the stages need.
-__device__ __forceinline__ int lane_now() {
-  int lane = threadIdx.x & 63;
-  asm volatile("" : "+v"(lane));
-  return lane;
-}
-
-// The kernel's arguments, read afresh, for the same reason: what a part's start and end need of
+// The kernel's arguments, read afresh, as lane_now reads the lane's number: what a part's start and end need of
 // them is not to take the stages' scalar registers.
 __device__ __forceinline__ AttendArgs args_now() {
   uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
@@ -349,23 +326,6 @@ template <>
 struct QueryTerms<_Float16> {
   static constexpr int n = 2;
 };
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  bf16x2 v;
-  v[0] = static_cast<__bf16>(lo);
-  v[1] = static_cast<__bf16>(hi);
-  return __builtin_bit_cast(uint32_t, v);
-}
-
-__device__ __forceinline__ float across_rows_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-
-__device__ __forceinline__ float across_rows_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
 
 // ---------------------------------------------------------------- scores
 // Which dword of a half-row's codes product i of the scores takes from quarter `quad` of the lanes:
@@ -492,14 +452,6 @@ __device__ __forceinline__ void tame(uint32_t (&codes)[8], float (&scale)[8]) {
     codes[k] = wild ? 0 : codes[k];
     scale[k] = wild ? 1.0f : scale[k];
   }
-}
-
-// A value at a device address that is a multiple of four; an address out of LDS must say so, or the
-// load counts as one that may be of LDS and is waited for with those.
-template <typename T>
-__device__ __forceinline__ T load_global(uint64_t p) {
-  typedef T Packed __attribute__((aligned(4)));
-  return *reinterpret_cast<const __attribute__((address_space(1))) Packed*>(p);
 }
 
 // ---------------------------------------------------------------- the cache's rows, through LDS
@@ -651,61 +603,6 @@ struct Stage {
     }
   }
 };
-
-// ---------------------------------------------------------------- softmax
-// The reference that a row's weights are taken against may lag its maximum by this much (in
-// powers of two): the sums are only rescaled when some row's maximum has grown past it. (Weights
-// are up to 2^8 then, so a mean of V above 2^119 may pass f32 on its way.)
-constexpr float kSlack = 8.0f;
-
-// A row's running state: four lanes hold the same m and shift, and a part of the sum l each.
-struct Running {
-  float m = -INFINITY, l = 0.0f;
-
-  // What the weights are taken against; a row may have seen nothing yet.
-  __device__ __forceinline__ float shift() const { return m == -INFINITY ? 0.0f : m; }
-};
-
-// The scores of tokens that a row does not see, and of those that are none, masked: `ahead` is the
-// number of tokens from this lane's first of the 32 up to the row's last, `ok` has a bit a token.
-template <int kTiles>
-__device__ __forceinline__ void mask(float (&s)[kTiles][8], const int (&ahead)[kTiles],
-                                     uint32_t ok) {
-#pragma unroll
-  for (int k = 0; k < 8; k++) {
-    const int at = 16 * (k >> 2) + (k & 3);
-    const bool in = (ok >> at) & 1;
-#pragma unroll
-    for (int n = 0; n < kTiles; n++) s[n][k] = ahead[n] >= at && in ? s[n][k] : -INFINITY;
-  }
-}
-
-// Whether eight new scores of each of this lane's rows (masked ones -infinity) take some row's
-// maximum too far past its reference: then all sums so far must be multiplied by `fade`.
-template <int kTiles>
-__device__ __forceinline__ bool grow(const float (&s)[kTiles][8], float scale_log2,
-                                     Running (&r)[kTiles], float (&fade)[kTiles]) {
-  float top[kTiles];
-  bool far = false;
-#pragma unroll
-  for (int n = 0; n < kTiles; n++) {
-    float x = s[n][0];
-#pragma unroll
-    for (int k = 1; k < 8; k++) x = fmaxf(x, s[n][k]);
-    top[n] = x * scale_log2;
-    far |= top[n] > r[n].m + kSlack;
-  }
-  if (__builtin_amdgcn_ballot_w64(far) == 0) return false;
-#pragma unroll
-  for (int n = 0; n < kTiles; n++) {
-    const float m = fmaxf(across_rows_max(top[n]), r[n].m);
-    const float before = r[n].m;
-    r[n].m = m;
-    fade[n] = __builtin_amdgcn_exp2f(before - r[n].shift());
-    r[n].l *= fade[n];
-  }
-  return true;
-}
 
 // Eight scores of this lane's row to weights.
 template <int kTerms>

@@ -12,7 +12,7 @@
 // or 2^127 are past f32 and bf16, and become infinities; no write makes those scales.)
 #pragma once
 
-#include "common.hpp"
+#include "softmax.hpp"
 
 namespace evs {
 
@@ -73,12 +73,6 @@ inline int fp4_cache(const char* who, const void* cache, int64_t num_blocks, int
   c.NG = static_cast<int32_t>(fp4_groups(d));
   return EVS_OK;
 }
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __builtin_bit_cast(float, byte << 23);  // 255 gives an exponent that converts to NaN

@@ -1,0 +1,307 @@
+// Attention over a paged cache at full width (bf16 or f16), whose sequences may share prefixes: what
+// its kernels share.
+//
+// The context of a query row (a query token and one of the heads that share a KV head) is its
+// group's prefix and then its sequence's own tokens up to the query's. With s_t the scaled product
+// of the query with token t's key,
+//
+//   out = sum_t exp(s_t - m) V_t / sum_t exp(s_t - m),   m = max_t s_t,   lse = m + ln(sum)
+//
+// and the sums over disjoint parts of the context join by their maxima: with (m_i, l_i, o_i) of part
+// i and m = max m_i, l = sum l_i exp(m_i - m) and likewise o. So a prefix is taken once for the rows
+// of all sequences of its group, and long contexts by several workgroups at once.
+//
+// Both products are MFMA tiles with f32 sums, computed transposed so that no value changes lanes
+// between them: the scores leave a lane with four tokens of one query row, and those weights are its
+// part of the second operand as they stand. A weight exp(s - m) is rounded to the cache's type before
+// it multiplies V (bf16: at most 2^-8 of it, f16: 2^-11 or, below 2^-14, 2^-25 in all); the sum of
+// the weights is taken before that.
+#pragma once
+
+#include <type_traits>
+
+#include "softmax.hpp"
+
+namespace evs {
+
+constexpr int kFullWaves = 4;
+constexpr int kFullThreads = 64 * kFullWaves;
+constexpr int kRowTile = 16;  // query rows that an MFMA tile has
+constexpr int kFullMinDim = 16;
+constexpr int kFullMaxDim = 256;
+
+// Contexts of one kind, in block tables.
+struct Contexts {
+  const int32_t* tables;
+  int64_t stride;
+  const int32_t* lens;
+  int32_t width, n;
+  int32_t chunk, splits;  // a part's tokens, and the most parts of a context
+  uint32_t tiles;         // row tiles that there may be
+};
+
+struct FullArgs {
+  char* base;
+  int64_t sb, so, sh, skv;  // page, slot in page, head, K to V, in bytes
+  int32_t num_blocks, block_size;
+  FastDiv div_bs;
+  int32_t heads, d;
+  const char* q;
+  int64_t q_token, q_head;  // strides in bytes
+  char* out;                // contiguous [tokens, q_heads, d]
+  float* lse;               // contiguous [tokens, q_heads], or null
+  float* top;               // the same in powers of two, for the weights, or null
+  const int32_t* starts;    // null: one query a sequence
+  int32_t seqs, tokens, max_q, q_heads;
+  FastDiv shared, div_heads;
+  float scale_log2;  // scale * log2(e)
+  Contexts own, pre;
+  const int32_t* group_starts;  // of the sequences of each prefix
+  // parts: sums [slots, tokens, q_heads, d], maxima and totals [slots, tokens, q_heads, 2]; the
+  // prefix's parts first
+  float* sums;
+  float* stats;
+  bool joined;  // rows are joined from parts
+  float* mass;  // [num_blocks, heads, block_size], or null
+};
+
+// Rows of queries and a context.
+struct Rows {
+  int32_t q0, nq;  // query tokens
+  int32_t rows;    // query rows of a KV head
+  int32_t len;     // tokens of the context
+};
+
+__device__ __forceinline__ int32_t length_of(const FullArgs& a, const Contexts& c, int i) {
+  const int64_t room = static_cast<int64_t>(c.width) * a.block_size;
+  const int32_t len = max(c.lens[i], 0);
+  return a.num_blocks == 0 ? 0 : len > room ? static_cast<int32_t>(room) : len;
+}
+
+// Sequence s and its own tokens, kept within the arguments' bounds.
+__device__ __forceinline__ Rows sequence_rows(const FullArgs& a, int s) {
+  Rows r;
+  if (a.starts == nullptr) {
+    r.q0 = s;
+    r.nq = 1;
+  } else {
+    r.q0 = max(a.starts[s], 0);
+    r.nq = min(a.starts[s + 1], a.tokens) - r.q0;
+    r.nq = max(min(r.nq, a.max_q), 0);
+  }
+  r.rows = r.nq * static_cast<int32_t>(a.shared.d);
+  r.len = length_of(a, a.own, s);
+  return r;
+}
+
+// The queries of group g's sequences, and its prefix.
+__device__ __forceinline__ Rows group_rows(const FullArgs& a, int g) {
+  const int s0 = min(max(a.group_starts[g], 0), a.seqs);
+  const int s1 = min(max(a.group_starts[g + 1], s0), a.seqs);
+  Rows r;
+  r.q0 = a.starts == nullptr ? s0 : min(max(a.starts[s0], 0), a.tokens);
+  const int end = a.starts == nullptr ? s1 : min(a.starts[s1], a.tokens);
+  r.nq = max(end - r.q0, 0);
+  r.rows = r.nq * static_cast<int32_t>(a.shared.d);
+  r.len = length_of(a, a.pre, g);
+  return r;
+}
+
+__device__ __forceinline__ Rows scalar_rows(Rows r) {
+  r.q0 = __builtin_amdgcn_readfirstlane(r.q0);
+  r.nq = __builtin_amdgcn_readfirstlane(r.nq);
+  r.rows = __builtin_amdgcn_readfirstlane(r.rows);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
+  return r;
+}
+
+// Parts of the first `end` tokens of a context; the last that there may be takes the rest.
+__device__ __forceinline__ int32_t parts_of(const Contexts& c, int32_t end) {
+  return end <= 0 ? 0 : min((end - 1) / c.chunk + 1, c.splits);
+}
+
+// The one of `n` with place `at` on a line on which each has count(i) places, found by the whole
+// workgroup of kFullThreads; false past the line's end.
+template <typename Count>
+__device__ __forceinline__ bool find_place(uint32_t n, uint32_t at, Count count, uint32_t& who,
+                                           uint32_t& place) {
+  __shared__ uint32_t s_wave[kFullWaves];
+  __shared__ uint32_t s_who, s_place;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t before = 0;
+  for (uint32_t i0 = 0; i0 < n; i0 += kFullThreads) {
+    const uint32_t i = i0 + tid;
+    const uint32_t mine = i < n ? count(i) : 0;
+    uint32_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t up = __shfl_up(sum, d);
+      if (lane >= static_cast<uint32_t>(d)) sum += up;
+    }
+    if (lane == 63) s_wave[wave] = sum;
+    __syncthreads();
+    uint32_t from = before + sum - mine;
+    for (uint32_t k = 0; k < kFullWaves; k++) {
+      if (k < wave) from += s_wave[k];
+      before += s_wave[k];
+    }
+    if (at >= from && at - from < mine) {
+      s_who = i;
+      s_place = at - from;
+    }
+    __syncthreads();
+    if (at < before) {
+      who = __builtin_amdgcn_readfirstlane(s_who);
+      place = __builtin_amdgcn_readfirstlane(s_place);
+      return true;
+    }
+  }
+  return false;
+}
+
+// The last of the ascending at[0], ..., at[n - 1] that is at most x, by a wave; -1 if there is none.
+__device__ __forceinline__ int last_at_most(const int32_t* at, int n, int x) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, span = n;
+  while (span > 0) {
+    const int step = (span + 63) >> 6;
+    const int i = lane * step;
+    const bool below = i < span && at[lo + i] <= x;
+    const int k = __popcll(__builtin_amdgcn_ballot_w64(below));
+    if (k == 0) return lo - 1;
+    lo += (k - 1) * step;
+    span -= (k - 1) * step;
+    span = span < step ? span : step;
+    if (span == 1) return lo;
+  }
+  return -1;
+}
+
+// The sequence that names query `token`, by a wave; -1 if none does.
+__device__ __forceinline__ int sequence_of(const FullArgs& a, int token) {
+  if (a.starts == nullptr) return token < a.seqs ? token : -1;
+  const int s = __builtin_amdgcn_readfirstlane(last_at_most(a.starts, a.seqs, token));
+  if (s < 0) return -1;
+  const Rows r = scalar_rows(sequence_rows(a, s));
+  return token >= r.q0 && token - r.q0 < r.nq ? s : -1;
+}
+
+// The group of sequence s, by a wave; -1 if it has no prefix.
+__device__ __forceinline__ int group_of(const FullArgs& a, int s) {
+  if (a.pre.n == 0) return -1;
+  const int g = __builtin_amdgcn_readfirstlane(last_at_most(a.group_starts, a.pre.n, s));
+  return g >= 0 && s < a.group_starts[g + 1] ? g : -1;
+}
+
+// ---------------------------------------------------------------- products
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// D[16, 16] += A[16, 32] B[32, 16]: lane l has eight elements of A's row l % 16 and of B's column
+// l % 16, from 8 (l / 16) on, and of D's column l % 16 the rows 4 (l / 16) to + 3.
+template <typename T>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __bf16>::value) {
+    return pack_bf16(lo, hi);
+  } else {
+    f16x2 v;
+    v[0] = static_cast<_Float16>(lo);
+    v[1] = static_cast<_Float16>(hi);
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// The bits of a half-word that are all set in an infinity and a NaN.
+template <typename T>
+constexpr uint32_t kWildBits = std::is_same<T, __bf16>::value ? 0x7F80u : 0x7C00u;
+
+// A dword's two values without those that are no finite numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t tamed(uint32_t x) {
+  constexpr uint32_t lo = kWildBits<T>, hi = kWildBits<T> << 16;
+  x = (x & lo) == lo ? x & 0xFFFF0000u : x;
+  return (x & hi) == hi ? x & 0xFFFFu : x;
+}
+template <typename T>
+__device__ __forceinline__ bool is_wild(uint32_t x) {
+  constexpr uint32_t lo = kWildBits<T>, hi = kWildBits<T> << 16;
+  return (x & lo) == lo || (x & hi) == hi;
+}
+
+// 16 bytes of a row that starts on 16.
+__device__ __forceinline__ u32x4 load16(uint64_t p) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(p);
+}
+__device__ __forceinline__ u32x2 load8(uint64_t p) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) u32x2*>(p);
+}
+
+// A query row's chunks of eight elements 4 i + quad, as operands; zeros past its end.
+template <int NG>
+__device__ __forceinline__ void load_query(const FullArgs& a, const char* p, int quad,
+                                           u32x4 (&q)[NG]) {
+#pragma unroll
+  for (int i = 0; i < NG; i++) {
+    const int c = 4 * i + quad;
+    const bool in = 8 * c < a.d;
+    const u32x4 x = load16(reinterpret_cast<uint64_t>(p) + (in ? 16 * c : 0));
+#pragma unroll
+    for (int k = 0; k < 4; k++) q[i][k] = in ? x[k] : 0;
+  }
+}
+
+// Eight scores of this lane's row to weights, as an operand.
+template <typename T>
+__device__ __forceinline__ u32x4 full_weights(const float (&s)[8], float scale_log2, Running& r) {
+  const float shift = r.shift();
+  u32x4 p;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], scale_log2, -shift));
+    const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k + 1], scale_log2, -shift));
+    r.l += lo + hi;
+    p[k / 2] = pack2<T>(lo, hi);
+  }
+  return p;
+}
+
+// ---------------------------------------------------------------- results
+// Where a part's row lies.
+__device__ __forceinline__ int64_t part_at(const FullArgs& a, int32_t slot, int32_t token,
+                                           int32_t q_head) {
+  return (static_cast<int64_t>(slot) * a.tokens + token) * a.q_heads + q_head;
+}
+
+// Four elements of an output row, 4 w on, from the sums, their reference and the weights' total.
+template <typename T>
+__device__ __forceinline__ void finish4(const FullArgs& a, int32_t token, int32_t q_head, int w,
+                                        f32x4 v, float top, float total) {
+  const float inv = total > 0 ? 1.0f / total : (total == 0 ? 0.0f : total);  // NaN stays
+  const int64_t at = static_cast<int64_t>(token) * a.q_heads + q_head;
+  u32x2 y;
+  y[0] = pack2<T>(v[0] * inv, v[1] * inv);
+  y[1] = pack2<T>(v[2] * inv, v[3] * inv);
+  *reinterpret_cast<u32x2*>(a.out + (at * a.d + 4 * w) * 2) = y;
+  if (w == 0) {
+    const float log2 = total == 0 ? -INFINITY : top + __builtin_amdgcn_logf(total);
+    if (a.lse != nullptr) a.lse[at] = log2 * kLn2;
+    // a row that sees nothing gives nothing
+    if (a.top != nullptr) a.top[at] = total == 0 ? INFINITY : log2;
+  }
+}
+
+int full_rows(const FullArgs& a, int type, hipStream_t s);
+int full_weigh(const FullArgs& a, int type, int64_t max_len, int64_t max_prefix, hipStream_t s);
+
+}  // namespace evs

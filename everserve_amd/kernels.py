@@ -264,6 +264,14 @@ _SIGNATURES: tuple[tuple[str, object, tuple], ...] = (
     ("evs_plan_compaction_workspace", _I32, (_I64, _P)),
     ("evs_plan_compaction", _I32,
      (_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _I64, _P)),
+    ("evs_attend_workspace", _I32,
+     (_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _P)),
+    ("evs_attend", _I32,
+     (_P, _P, _I32, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P,
+      _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P)),
+    ("evs_evict", _I32,
+     (_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64,
+      _I64, _P, _P, _P, _P)),
 )
 ENTRY_POINTS = tuple(name for name, _, _ in _SIGNATURES)
 
@@ -323,6 +331,16 @@ def _on_device_of(t):
     return _HERE if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
 
 
+def _table(t, what: str):
+    """``(address, row stride, rows, width)`` of block tables: int32 on the GPU, a row contiguous."""
+    import torch
+
+    if t.dim() != 2 or t.dtype != torch.int32 or not t.is_cuda or (
+            t.shape[1] > 1 and t.stride(1) != 1):
+        raise RuntimeError(f"{what} are int32 [rows, pages] on the device, a row contiguous")
+    return t.data_ptr(), t.stride(0), *t.shape
+
+
 def _device_ptr(t, what: str, dtype) -> int:
     """A device tensor's address, after checking it is on the GPU and of ``dtype``."""
     if t.is_cuda and t.dtype == dtype and t.is_contiguous():
@@ -332,6 +350,12 @@ def _device_ptr(t, what: str, dtype) -> int:
     if t.dtype != dtype:
         raise RuntimeError(f"{what} must be {dtype}, got {t.dtype}")
     raise RuntimeError(f"{what} must be contiguous")
+
+
+def _bound(given: int, room: int) -> int:
+    """A bound on lengths as the library takes it: the tables' room where none is given, or more."""
+    room = min(room, 2**31 - 1)
+    return min(int(given), room) if given else room
 
 
 def _one_device(what: str, *tensors) -> None:
@@ -365,7 +389,7 @@ class Kernels:
         self.MAX_ROWS, self.CTRL_WORDS, self.ABORT, self.LATE, self.BOUND = (int(w) for w in words)
         self._workspace: dict = {}  # order_pairs' workspace, per (device, stream)
         self._pairs: dict = {}  # scatter_rows' sorted pairs, per (device, stream)
-        self._attend_bytes: dict = {}  # fp4_attend's workspace sizes, by its counts
+        self._attend_bytes: dict = {}  # attend's and fp4_attend's workspace sizes, by their counts
 
     def _check(self, rc: int) -> None:
         if rc != EVS_OK:
@@ -889,6 +913,146 @@ class Kernels:
         if rc != EVS_OK:
             self._check(rc)
         return (out, lse) if return_lse else out
+
+    # -------------------------------------------------------------- full-width caches
+    def attend(self, q, cache, num_blocks: int, block_size: int, heads: int,
+               strides: Sequence[int], block_tables, seq_lens, q_starts=None,
+               max_q: int | None = None, scale: float | None = None, max_len: int = 0, out=None,
+               return_lse: bool = False, prefix=None, mass=None):
+        """Attention of ``q`` ([tokens, q_heads, d], the cache's bf16 or f16) over a full-width
+        ``cache``.
+
+        The arguments are :meth:`fp4_attend`'s, and more: ``prefix`` (a
+        :class:`everserve_amd.state.full.SharedPrefix`) has what groups of the sequences see ahead
+        of their own tokens, which ``block_tables`` and ``seq_lens`` then name alone; ``mass``
+        (f32 [num_blocks, heads, block_size], contiguous) gets each token's weight added, summed
+        over the rows that see it and the heads that share its KV head, the call's own new tokens
+        (each sequence's last, its queries') from 0 on: a page must not be named twice then.
+
+        Returns ``out`` ([tokens, q_heads, d], written into if given), with ``return_lse`` also the
+        f32 [tokens, q_heads] logs of the sums of exp(scores). A row that sees nothing is zeros,
+        its log -infinity; a page id outside the cache holds nothing. There is no backward pass.
+        Enqueued on the current stream; its workspace comes from torch's allocator.
+
+        Scores, maxima and sums are f32; the weights that multiply V are rounded to the cache's
+        type. ``max_len`` and ``prefix.max_len`` steer how the work is split, as in
+        :meth:`fp4_attend`, which also says which rows are not written."""
+        import torch
+
+        type_ = _row_types().get(q.dtype, 2)
+        if q.dim() != 3 or type_ == 2 or not q.is_cuda or q.dtype != cache.dtype:
+            raise RuntimeError(f"attend: queries are [tokens, heads, d] of the cache's type, bf16 "
+                               f"or f16, on the device, not {q.dtype} of shape {tuple(q.shape)}")
+        if torch.is_grad_enabled() and (q.requires_grad or cache.requires_grad):
+            raise RuntimeError("attend: no backward pass: detach the queries and the cache")
+        tokens, q_heads, d = q.shape
+        qs = q.stride()
+        if qs[2] != 1:
+            raise RuntimeError("attend: a query's elements must be contiguous")
+        tp, tstride, seqs, width = _table(block_tables, "attend: block_tables")
+        lp = _device_ptr(seq_lens, "attend: seq_lens", torch.int32)
+        if seq_lens.numel() != seqs:
+            raise RuntimeError(f"attend: {seqs} block tables but {seq_lens.numel()} lengths")
+        starts = None
+        if q_starts is not None:
+            starts = _device_ptr(q_starts, "attend: q_starts", torch.int32)
+            if q_starts.numel() != seqs + 1:
+                raise RuntimeError(f"attend: {seqs} sequences need {seqs + 1} query starts, got "
+                                   f"{q_starts.numel()}")
+        if max_q is None:
+            max_q = 1 if q_starts is None else tokens
+        if not cache.is_cuda:
+            raise RuntimeError("attend: the cache must be on the device")
+        pp = pl = ps = None
+        pstride = groups = pwidth = max_prefix = 0
+        if prefix is not None:
+            pp, pstride, groups, pwidth = _table(prefix.block_tables, "attend: a prefix's tables")
+            pl = _device_ptr(prefix.lens, "attend: a prefix's lens", torch.int32)
+            ps = _device_ptr(prefix.starts, "attend: a prefix's starts", torch.int32)
+            if prefix.lens.numel() != groups or prefix.starts.numel() != groups + 1:
+                raise RuntimeError(f"attend: {groups} prefixes need as many lengths and "
+                                   f"{groups + 1} starts of their sequences")
+            max_prefix = _bound(prefix.max_len, pwidth * block_size)
+            _one_device("attend", q, prefix.block_tables, prefix.lens, prefix.starts)
+        mp = None
+        if mass is not None:
+            mp = _device_ptr(mass, "attend: mass", torch.float32)
+            if tuple(mass.shape) != (num_blocks, heads, block_size):
+                raise RuntimeError(f"attend: mass of shape {tuple(mass.shape)}, expected "
+                                   f"{(num_blocks, heads, block_size)}")
+        idle = seqs == 0 or max_q == 0  # no row is written
+        if out is None:
+            new = torch.zeros if idle else torch.empty
+            out = new((tokens, q_heads, d), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise RuntimeError("attend: out must be contiguous and like the queries")
+        lse = None
+        if return_lse:
+            lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
+            if idle:
+                lse.fill_(-math.inf)
+        _one_device("attend", q, cache, block_tables, seq_lens, q_starts, out, mass)
+        max_len = _bound(max_len, width * block_size)
+        counts = (seqs, tokens, q_heads, heads, d, max_q, max_len, groups, max_prefix,
+                  mass is not None)
+        with _on_device_of(q):
+            need = self._attend_bytes.get(counts)
+            if need is None:
+                size = ctypes.c_int64()
+                self._check(self._lib.evs_attend_workspace(*counts, ctypes.byref(size)))
+                if len(self._attend_bytes) >= 4096:  # the same counts come back in a serving loop
+                    self._attend_bytes.clear()
+                need = self._attend_bytes[counts] = size.value
+            device = q.device
+            work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            rc = self._lib.evs_attend(
+                q.data_ptr(), _TWO(qs[0], qs[1]), type_, out.data_ptr(),
+                lse.data_ptr() if return_lse else None, tokens, q_heads, cache.data_ptr(),
+                num_blocks, block_size, heads, d, _five(strides), tp, tstride, width, lp, starts,
+                seqs, max_q, max_len, pp, pstride, pwidth, pl, ps, groups, max_prefix, mp,
+                d ** -0.5 if scale is None else scale, work.data_ptr() if need else None, need,
+                _stream_of(device))
+        if rc != EVS_OK:
+            self._check(rc)
+        return (out, lse) if return_lse else out
+
+    def evict(self, layer_ptrs, num_blocks: int, heads: int, d: int, block_size: int,
+              strides: Sequence[int], elem_size: int, block_tables, seq_lens, new_tables,
+              budget: int, mass, recent: int = 0):
+        """Cut sequences to ``budget`` tokens in every layer and KV head and move the rows that stay
+        to new pages: new tensors ``(lens, kept)``, int32 [seqs] and [layers, seqs, heads, budget].
+
+        :meth:`everserve_amd.state.evict.Evictor.evict` says what stays; ``mass`` is f32 [layers,
+        num_blocks, heads, block_size], contiguous. Enqueued on the current stream."""
+        import torch
+
+        lp = _device_ptr(layer_ptrs, "evict: layer_ptrs", torch.long)
+        tp, tstride, seqs, width = _table(block_tables, "evict: block_tables")
+        np_, nstride, rows, new_width = _table(new_tables, "evict: new_tables")
+        sp = _device_ptr(seq_lens, "evict: seq_lens", torch.int32)
+        if rows != seqs or seq_lens.numel() != seqs:
+            raise RuntimeError(f"evict: {seqs} block tables, {rows} new ones and "
+                               f"{seq_lens.numel()} lengths")
+        mp = _device_ptr(mass, "evict: mass", torch.float32)
+        layers = layer_ptrs.numel()
+        if tuple(mass.shape) != (layers, num_blocks, heads, block_size):
+            raise RuntimeError(f"evict: mass of shape {tuple(mass.shape)}, expected "
+                               f"{(layers, num_blocks, heads, block_size)}")
+        _one_device("evict", layer_ptrs, block_tables, seq_lens, new_tables, mass)
+        budget, recent = int(budget), int(recent)
+        if not 0 <= recent <= budget:
+            raise RuntimeError(f"evict: {recent} newest tokens of a budget of {budget}")
+        device = mass.device
+        lens = torch.empty(seqs, dtype=torch.int32, device=device)
+        kept = torch.empty((layers, seqs, heads, budget), dtype=torch.int32, device=device)
+        with _on_device_of(mass):
+            rc = self._lib.evs_evict(
+                lp, layers, num_blocks, heads, d, block_size, _five(strides), elem_size, tp,
+                tstride, width, sp, seqs, np_, nstride, new_width, budget, recent, mp,
+                lens.data_ptr(), kept.data_ptr(), _stream_of(device))
+        if rc != EVS_OK:
+            self._check(rc)
+        return lens, kept
 
     # -------------------------------------------------------------- pages of a cache
     def copy_blocks(self, layer_ptrs, src, dst, num_blocks: int, heads: int, d: int,

@@ -213,8 +213,9 @@ int evs_slot_all_reduce(const void* inp, void* out, int64_t n, const int64_t* bu
  * (core/csrc/slot.cu:229-232). Writes the count to *out. */
 int evs_slot_blocks(int64_t maxn, int64_t words, int64_t* out);
 
-/* ---- A paged cache held in 4 bits, and the pages of any cache. None of these has a counterpart in
- * the reference, whose caches are its engine's. ----
+/* ---- A paged cache held in 4 bits, the pages of any cache, attention over full-width ones and
+ * eviction from any. None of these has a counterpart in the reference, whose caches are its engine's.
+ * ----
  *
  * A 4-bit half-row is the K or the V of one slot and head, head_dim elements (a multiple of 8, 16 to
  * 256): head_dim / 2 bytes of E2M1 codes (element j in bits 4 (j % 8) of dword j / 8), one scale
@@ -303,6 +304,65 @@ int evs_plan_compaction(const int32_t* tables, int64_t rows, int64_t width, int6
                         const int32_t* counts, int64_t num_blocks, int32_t* tables_out,
                         int32_t* src, int32_t* dst, int64_t room, int32_t* sizes,
                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of query rows over a paged cache at full width, whose sequences may share prefixes.
+ * Sequence s has its own first lens[s] tokens in the pages tables[s] (as evs_fp4_attend's), and the
+ * queries q_starts[s] .. q_starts[s + 1] - 1, which are the last of them. Group g of `groups` (0: no
+ * prefixes) has the sequences group_starts[g] .. group_starts[g + 1] - 1 (device, int32 [groups + 1],
+ * ascending), and ahead of their own tokens all of them see the prefix_lens[g] tokens (device, int32)
+ * in the pages prefix_tables[g] (device, int32, rows of prefix_width entries, prefix_stride apart),
+ * which are read once for the whole group. A sequence of no group sees its own tokens alone.
+ *   cache   elements of `type` (EVS_BF16 or EVS_F16), strides in elements as for evs_gather_rows,
+ *           the last 1; head_dim a multiple of 8, 16 to 256; rows start on 16 bytes;
+ *   q       [tokens, q_heads, head_dim] of `type`, contiguous in the last; q_strides: token and head
+ *           strides in elements; rows start on 16 bytes;
+ *   out     contiguous [tokens, q_heads, head_dim] of `type`, starting on 16 bytes;
+ *   lse     contiguous f32 [tokens, q_heads], the natural log of the sum of exp(scores), or NULL;
+ *   mass    contiguous f32 [num_blocks, heads, block_size], or NULL: the weight exp(score - lse) that
+ *           a slot's token gets from a row, summed over the rows that see it and the query heads that
+ *           share the KV head, is added to it. The tokens of the call's own queries (the last of
+ *           each sequence) start from 0. A page that two of the call's contexts name, or one names
+ *           twice, must be in no table when mass is given.
+ * Scores, maxima and sums are f32; a weight is rounded to `type` before it multiplies V. A row that
+ * sees nothing gives zeros, and lse -infinity. A value of V that is no finite number reaches the
+ * rows that see its token and no others. A table entry outside [0, num_blocks) holds nothing: its
+ * tokens are masked. Lengths are taken up to their tables' room, a sequence's queries up to max_q
+ * and `tokens`. Queries that no sequence names are not written. `max_len` and `max_prefix` (0: the
+ * tables' room) are at least the longest lengths, and only steer how the work is split.
+ * `workspace` is device memory of evs_attend_workspace bytes for the same counts (max_len and
+ * max_prefix as the call resolves them: the tables' room where they are 0 or above it), 16-byte
+ * aligned, that no overlapping call uses. The call allocates nothing and may be captured. */
+int evs_attend_workspace(int64_t seqs, int64_t tokens, int64_t q_heads, int64_t heads,
+                         int64_t head_dim, int64_t max_q, int64_t max_len, int64_t groups,
+                         int64_t max_prefix, int mass, int64_t* bytes);
+int evs_attend(const void* q, const int64_t* q_strides, int type, void* out, float* lse,
+               int64_t tokens, int64_t q_heads, const void* cache, int64_t num_blocks,
+               int64_t block_size, int64_t heads, int64_t head_dim, const int64_t* strides,
+               const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lens,
+               const int32_t* q_starts, int64_t seqs, int64_t max_q, int64_t max_len,
+               const int32_t* prefix_tables, int64_t prefix_stride, int64_t prefix_width,
+               const int32_t* prefix_lens, const int32_t* group_starts, int64_t groups,
+               int64_t max_prefix, float* mass, float scale, void* workspace,
+               int64_t workspace_bytes, void* stream);
+
+/* Cut sequences to `budget` tokens in every layer and KV head by the mass that their tokens gathered
+ * (evs_attend), and move the rows that stay to new pages. Of a sequence's lens[s] tokens (device,
+ * int32; tables as for evs_attend, of seqs rows) all stay if there are no more than the budget; else
+ * the `recent` last and of the others those with the largest mass[layer] (device, contiguous f32
+ * [num_layers, num_blocks, heads, block_size]), of equal ones the first (-0 equals 0, what is no
+ * number comes before all others, a token on a page outside the cache after them). They keep their
+ * order: the j-th goes to slot j % block_size of page new_tables[s][j / block_size], K, V and mass
+ * (caches addressed as in evs_copy_blocks, the elements of a row contiguous; any element type).
+ * lens_out[s] (device, int32) gets the tokens that stay, kept (device, contiguous int32 [num_layers,
+ * seqs, heads, budget]) which they are, -1 past them. The pages of `tables` are only read, so other
+ * sequences may share them; those of new_tables must be named once and in none of `tables`. Rows and
+ * mass from and to pages outside the cache are not moved. Two launches; nothing is allocated. */
+int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t num_blocks, int64_t num_heads,
+              int64_t head_dim, int64_t block_size, const int64_t* strides, int64_t elem_size,
+              const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lens,
+              int64_t seqs, const int32_t* new_tables, int64_t new_stride, int64_t new_width,
+              int64_t budget, int64_t recent, float* mass, int32_t* lens_out, int32_t* kept,
+              void* stream);
 
 /* Pin `bytes` of host memory at `ptr`, mapped into the device address space; *device_ptr receives
  * the address kernels use. Replaces host_register_mapped (core/csrc/gather.cu:137-144). */
