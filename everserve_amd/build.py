@@ -30,9 +30,9 @@ LIBRARY = "libeverserve_mi355x.so"
 STAMP = "stamp.json"
 SOURCES = ("rows.hip", "order.hip", "reduce.hip", "slot.hip", "host_rows.hip", "store.hip",
            "runtime.hip", "fp4.hip", "attend.hip", "attend_few.hip", "attend_many.hip",
-           "pages.hip", "full.hip", "full_rows.hip", "full_weigh.hip", "evict.hip")
-HEADERS = ("attend.hpp", "common.hpp", "fp4.hpp", "full.hpp", "host_copy.hpp", "softmax.hpp",
-           "workers.hpp")
+           "pages.hip", "full.hip", "full_attend.hip", "full_weigh.hip", "evict.hip")
+HEADERS = ("attend.hpp", "common.hpp", "fp4.hpp", "full.hpp", "full_rows.hpp",
+           "full_tiles.hpp", "host_copy.hpp", "softmax.hpp", "workers.hpp")
 PUBLIC_HEADERS = ("everserve_mi355x.h",)
 DEFAULT_ARCHS = "gfx950"
 # Flags for one source only. The local reduce's counting atomics run in one lane and their

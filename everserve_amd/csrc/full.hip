@@ -1,36 +1,52 @@
 // Attention over full-width pages: the calls, how their work is dealt out, and the join of contexts
-// in several parts (full.hpp has the mathematics, full_rows.hip and full_weigh.hip the kernels).
+// in several parts (full.hpp has the mathematics, full_attend.hip and full_weigh.hip the
+// kernels).
 #include "full.hpp"
 
 namespace evs {
 namespace {
 
-// A query's rows joined from their parts: a workgroup takes four elements a thread.
+// Rows of one query joined from their parts: four elements a thread, and the parts in turn to as many
+// threads as there may be parts for; the rest of a workgroup takes further heads. Bound by latency
+// where parts are many, else by their bytes.
 template <typename T>
-__global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a) {
+__global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a, int word_bits,
+                                                          int turn_bits) {
+  __shared__ f32x4 s_v[kFullThreads];
+  __shared__ float s_m[kFullThreads], s_l[kFullThreads];
   const int token = blockIdx.x;
   const int s = sequence_of(a, token);
   if (s < 0) return;  // uniform
-  const int g = group_of(a, s);
   const Rows sq = scalar_rows(sequence_rows(a, s));
-  const int words = a.d / 4;
-  const int x = blockIdx.y * kFullThreads + threadIdx.x;
-  const int q_head = x / words, w = x - q_head * words;
-  if (q_head >= a.q_heads) return;
+  const int tid = threadIdx.x;
+  const int w = tid & ((1 << word_bits) - 1);
+  const int turn = (tid >> word_bits) & ((1 << turn_bits) - 1);
+  const int heads_at = kFullThreads >> (word_bits + turn_bits);
+  const int q_head = blockIdx.y * heads_at + (tid >> (word_bits + turn_bits));
   const int shared = a.shared.d;
-  // the row's tile sees the tokens up to its last row's
-  const int row = (token - sq.q0) * shared + q_head % shared;
-  const int last = min(row / kRowTile * kRowTile + kRowTile, sq.rows) - 1;
-  const int end = min(sq.len, sq.len - sq.nq + last / shared + 1);
-  const int before = g < 0 ? 0 : parts_of(a.pre, length_of(a, a.pre, g));
-  const int own = max(parts_of(a.own, end), 1);
+  // the tokens that the row's tile sees, and its parts
+  const bool few = sq.rows <= kRowTile, alone = sq.rows > kTogether;
+  const int g = a.group.tiles > 0 || (alone && a.pre.n > 0) ? group_of(a, s) : -1;
+  const int prefix = g < 0 ? 0 : length_of(a, a.pre, g);
+  const int ahead = alone ? prefix : 0;
+  const int in = min(q_head, a.q_heads - 1);
+  const int row = (token - sq.q0) * shared + in % shared;
+  const int tile = few ? kRowTile : kRowTile * kFullWaves * a.row_tiles;
+  const int last = min(row / tile * tile + tile, sq.rows) - 1;
+  const int end = min(ahead + sq.len, max(ahead + sq.len - sq.nq + last / shared + 1, ahead));
+  const Cut& cut = few ? a.few : a.many;
+  const bool joined = q_head < a.q_heads && is_joined(a, cut, sq.rows, end);
+  const int before = alone || !joined ? 0 : parts_of(a.group, prefix);
+  const int parts = joined ? before + max(parts_of(cut, end), 1) : 0;
   float top = -INFINITY, total = 0;
   f32x4 v = {0, 0, 0, 0};
-  for (int k = 0; k < before + own; k++) {
-    const int slot = k < before ? k : a.pre.splits + k - before;
-    const int64_t at = part_at(a, slot, token, q_head);
+  const int wr = min(w, a.d / 4 - 1);
+#pragma unroll 4
+  for (int k = turn; k < parts; k += 1 << turn_bits) {
+    const int slot = k < before ? k : a.group.splits + k - before;
+    const int64_t at = part_at(a, slot, token, in);
     const float m = a.stats[2 * at], l = a.stats[2 * at + 1];
-    const f32x4 y = *reinterpret_cast<const f32x4*>(a.sums + at * a.d + 4 * w);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(a.sums + at * a.d + 4 * wr);
     const float now = fmaxf(top, m);
     const float ref = now == -INFINITY ? 0.0f : now;
     const float f = __builtin_amdgcn_exp2f(top - ref), h = __builtin_amdgcn_exp2f(m - ref);
@@ -38,7 +54,24 @@ __global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a) {
     total = total * f + l * h;
     v = v * f + y * h;
   }
-  finish4<T>(a, token, q_head, w, v, top, total);
+  if (turn_bits > 0) {
+    s_v[tid] = v;
+    s_m[tid] = top;
+    s_l[tid] = total;
+    __syncthreads();
+    if (turn != 0) return;
+    for (int k = 1; k < 1 << turn_bits; k++) top = fmaxf(top, s_m[tid + (k << word_bits)]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    total = 0;
+    v = f32x4{0, 0, 0, 0};
+    for (int k = 0; k < 1 << turn_bits; k++) {
+      const int t = tid + (k << word_bits);
+      const float f = __builtin_amdgcn_exp2f(s_m[t] - ref);
+      total += s_l[t] * f;
+      v += s_v[t] * f;
+    }
+  }
+  if (joined && w < a.d / 4) finish4<T>(a, token, q_head, w, v, top, total);
 }
 
 __global__ __launch_bounds__(kFullThreads) void no_weights(float* top, int64_t n) {
@@ -49,21 +82,26 @@ __global__ __launch_bounds__(kFullThreads) void no_weights(float* top, int64_t n
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
 
-constexpr int64_t kFill = 1024;     // workgroups that fill the GPU
-constexpr int64_t kRound = 256;     // tokens that a workgroup's waves take in turn
+constexpr int64_t kRound = 256;  // tokens that a workgroup's waves take in turn, of few rows
+constexpr int64_t kFillRows = 1024;  // workgroups that fill the GPU, of few rows
+constexpr int64_t kFillTiles = 256;  // and of many
 constexpr int64_t kMostParts = 64;
 
-// How contexts of up to max_len tokens are cut: `tiles` row tiles of them there may be.
-void cut(Contexts& c, int64_t tiles, int64_t heads, int64_t max_len) {
-  c.tiles = static_cast<uint32_t>(tiles);
-  int64_t parts = ceil_div(kFill, tiles * heads);
-  parts = least(least(parts, kMostParts), ceil_div(max_len, kRound));
+// How contexts of up to max_len tokens are cut for `tiles` row tiles that there may be: into parts
+// that make `fill` workgroups in all, of `least_chunk` tokens at least.
+Cut cut(int64_t tiles, int64_t heads, int64_t max_len, int64_t fill, int64_t least_chunk) {
+  Cut c{};
+  if (tiles == 0) return c;
+  int64_t parts = least(least(ceil_div(fill, tiles * heads), kMostParts),
+                        ceil_div(max_len, least_chunk));
   parts = parts < 1 ? 1 : parts;
   int64_t chunk = ceil_div(ceil_div(max_len, parts), kRound) * kRound;
   chunk = chunk < kRound ? kRound : least(chunk, (int64_t{1} << 31) - kRound);
+  c.tiles = static_cast<uint32_t>(least(tiles, (int64_t{1} << 31) - 1));
   c.chunk = static_cast<int32_t>(chunk);
   c.splits = static_cast<int32_t>(least(ceil_div(max_len, chunk), kMostParts));
   if (c.splits < 1) c.splits = 1;
+  return c;
 }
 
 struct Counts {
@@ -81,7 +119,9 @@ bool good(const Counts& n) {
 }
 
 struct Deal {
-  Contexts own, pre;
+  Cut group, few, many;
+  bool few_groups;
+  int row_tiles;
   int64_t slots, sums, stats, top, bytes;
 };
 
@@ -89,19 +129,35 @@ Deal deal(Counts n) {
   Deal r{};
   const int64_t shared = n.q_heads / n.heads;
   if (n.max_q > n.tokens) n.max_q = n.tokens;
-  const int64_t each = ceil_div(n.max_q * shared, kRowTile);
-  cut(r.own, n.max_q == 1 ? n.seqs * each
-                          : least(n.seqs * each, n.tokens * shared / kRowTile + n.seqs),
-      n.heads, n.max_len);
-  if (n.groups > 0) cut(r.pre, n.tokens * shared / kRowTile + n.groups, n.heads, n.max_prefix);
-  r.slots = r.pre.splits + r.own.splits;
+  const int64_t most = n.max_q * shared, rows = n.tokens * shared;  // of a sequence, of a KV head
+  const bool together = n.groups > 0 && shared <= kTogether;
+  r.few_groups = rows <= kRowTile;
+  // tiles of 128 rows where some context has them; wide heads leave no registers for them
+  const bool wide = n.d <= 128 && (most > kTogether || (together && rows / n.groups > kTogether));
+  r.row_tiles = wide ? 2 : 1;
+  const int64_t tile = kRowTile * kFullWaves * r.row_tiles;
+  if (shared <= kRowTile) r.few = cut(n.seqs, n.heads, n.max_len, kFillRows, kRound);
+  if (most > kRowTile)
+    r.many = cut(least(n.seqs * ceil_div(most, tile),
+                       rows / tile + least(n.seqs, rows / (kRowTile + 1))),
+                 n.heads, n.max_len + n.max_prefix, kFillTiles, 2 * kRound);
+  if (together)
+    r.group = r.few_groups ? cut(n.groups, n.heads, n.max_prefix, kFillRows, kRound)
+                           : cut(rows / tile + n.groups, n.heads, n.max_prefix, kFillTiles, kRound);
+  r.slots = r.group.splits + (r.few.splits > r.many.splits ? r.few.splits : r.many.splits);
   if (r.slots == 1) r.slots = 0;
-  const int64_t rows = n.tokens * n.q_heads;
-  r.sums = r.slots * rows * n.d * 4;
-  r.stats = r.slots * rows * 8;
-  r.top = n.mass ? rows * 4 : 0;
+  const int64_t every = n.tokens * n.q_heads;
+  r.sums = r.slots * every * n.d * 4;
+  r.stats = r.slots * every * 8;
+  r.top = n.mass ? every * 4 : 0;
   r.bytes = (r.sums + r.stats + r.top + 15) / 16 * 16;
   return r;
+}
+
+// Workgroups of the launch, as full_attend has them.
+int64_t workgroups(const Deal& r, int64_t heads) {
+  const auto in = [&](const Cut& c) { return (c.splits * heads + 7) / 8 * 8 * c.tiles; };
+  return in(r.group) + in(r.few) + in(r.many);
 }
 
 // What a length may be at most where the caller does not say.
@@ -181,8 +237,7 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   const evs::Deal deal = evs::deal(n);
   // (a launch has at most 2^32 - 1 threads along x)
   EVS_REQUIRE(tokens < most / 256 &&
-                  (static_cast<int64_t>(deal.own.tiles) * deal.own.splits +
-                   static_cast<int64_t>(deal.pre.tiles) * deal.pre.splits) * heads < most / 256,
+                  evs::workgroups(deal, heads) < most / 256,
               "%s: too many tiles of query rows", who);
   EVS_REQUIRE(deal.bytes <= workspace_bytes &&
                   (deal.bytes == 0 || (workspace != nullptr &&
@@ -213,13 +268,16 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   a.shared = evs::FastDiv(static_cast<uint32_t>(q_heads / heads));
   a.div_heads = evs::FastDiv(static_cast<uint32_t>(heads));
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.own = deal.own;
+  a.group = deal.group;
+  a.few = deal.few;
+  a.many = deal.many;
+  a.few_groups = deal.few_groups;
+  a.row_tiles = deal.row_tiles;
   a.own.tables = tables;
   a.own.stride = table_stride;
   a.own.width = static_cast<int32_t>(width);
   a.own.lens = lens;
   a.own.n = a.seqs;
-  a.pre = deal.pre;
   if (groups > 0) {
     a.pre.tables = prefix_tables;
     a.pre.stride = prefix_stride;
@@ -231,7 +289,6 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   char* at = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<float*>(at);
   a.stats = reinterpret_cast<float*>(at + deal.sums);
-  a.joined = deal.slots > 0;
   if (mass != nullptr) {
     a.mass = mass;
     a.top = reinterpret_cast<float*>(at + deal.sums + deal.stats);
@@ -244,15 +301,18 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
                                                                                           rows);
     EVS_LAUNCHED(who);
   }
-  if (const int rc = evs::full_rows(a, type, s)) return rc;
-  if (a.joined) {
+  if (const int rc = evs::full_attend(a, type, s)) return rc;
+  if (deal.slots > 0) {
+    int word_bits = 0, turn_bits = 0;
+    while ((4 << word_bits) < head_dim) word_bits++;
+    while (word_bits + turn_bits < 8 && (4 << turn_bits) < deal.slots) turn_bits++;
+    const int64_t heads_at = evs::kFullThreads >> (word_bits + turn_bits);
     const dim3 grid(static_cast<uint32_t>(tokens),
-                    static_cast<uint32_t>((q_heads * head_dim / 4 + evs::kFullThreads - 1) /
-                                          evs::kFullThreads));
+                    static_cast<uint32_t>((q_heads + heads_at - 1) / heads_at));
     if (type == EVS_BF16)
-      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a);
+      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a, word_bits, turn_bits);
     else
-      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a);
+      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a, word_bits, turn_bits);
     EVS_LAUNCHED(who);
   }
   return mass == nullptr ? EVS_OK : evs::full_weigh(a, type, n.max_len, n.max_prefix, s);

@@ -27,6 +27,10 @@ namespace evs {
 constexpr int kFullWaves = 4;
 constexpr int kFullThreads = 64 * kFullWaves;
 constexpr int kRowTile = 16;  // query rows that an MFMA tile has
+// Sequences of up to kRowTile query rows a KV head take their own tokens in full_rows.hpp, others in
+// full_tiles.hpp; those of up to kTogether take a prefix with the rest of their group, and longer
+// chunks, which fill tiles by themselves, take it ahead of their own tokens, as one context.
+constexpr int kTogether = 64;
 constexpr int kFullMinDim = 16;
 constexpr int kFullMaxDim = 256;
 
@@ -36,6 +40,10 @@ struct Contexts {
   int64_t stride;
   const int32_t* lens;
   int32_t width, n;
+};
+
+// How contexts are cut into parts, one a workgroup.
+struct Cut {
   int32_t chunk, splits;  // a part's tokens, and the most parts of a context
   uint32_t tiles;         // row tiles that there may be
 };
@@ -57,11 +65,14 @@ struct FullArgs {
   float scale_log2;  // scale * log2(e)
   Contexts own, pre;
   const int32_t* group_starts;  // of the sequences of each prefix
+  // how prefixes are cut for their groups' rows, own tokens for few rows, and contexts for many
+  Cut group, few, many;
+  bool few_groups;  // a group has at most kRowTile rows
   // parts: sums [slots, tokens, q_heads, d], maxima and totals [slots, tokens, q_heads, 2]; the
   // prefix's parts first
   float* sums;
   float* stats;
-  bool joined;  // rows are joined from parts
+  int32_t row_tiles;  // of 16 rows, that a wave has of a tile of many
   float* mass;  // [num_blocks, heads, block_size], or null
 };
 
@@ -116,8 +127,15 @@ __device__ __forceinline__ Rows scalar_rows(Rows r) {
 }
 
 // Parts of the first `end` tokens of a context; the last that there may be takes the rest.
-__device__ __forceinline__ int32_t parts_of(const Contexts& c, int32_t end) {
+__device__ __forceinline__ int32_t parts_of(const Cut& c, int32_t end) {
   return end <= 0 ? 0 : min((end - 1) / c.chunk + 1, c.splits);
+}
+
+// Whether rows of a sequence with `rows` of them, whose own part of the context ends at `end`, are
+// joined from parts. Of one part, without a prefix that others share, they are written where they go.
+__device__ __forceinline__ bool is_joined(const FullArgs& a, const Cut& c, int32_t rows,
+                                          int32_t end) {
+  return parts_of(c, end) > 1 || (rows <= kTogether && a.group.tiles > 0);
 }
 
 // The one of `n` with place `at` on a line on which each has count(i) places, found by the whole
@@ -301,7 +319,72 @@ __device__ __forceinline__ void finish4(const FullArgs& a, int32_t token, int32_
   }
 }
 
-int full_rows(const FullArgs& a, int type, hipStream_t s);
+// Four sums of a row: to its part if it is joined, else to the output.
+template <typename T>
+__device__ __forceinline__ void put4(const FullArgs& a, bool joined, int32_t slot, int32_t token,
+                                     int32_t q_head, int w, f32x4 v, float top, float total) {
+  if (joined) {
+    const int64_t at = part_at(a, slot, token, q_head);
+    *reinterpret_cast<f32x4*>(a.sums + at * a.d + 4 * w) = v;
+    if (w == 0) {
+      a.stats[2 * at] = top;
+      a.stats[2 * at + 1] = total;
+    }
+  } else {
+    finish4<T>(a, token, q_head, w, v, top, total);
+  }
+}
+
+// The products of the values that are no finite numbers among 32 tokens, whose rows are at `at` and
+// whose scores for this lane's row are `s`: the row's elements get them if it sees the token, of
+// which it sees those up to `ahead`. Such values are kept out of the other products, where a row
+// ahead of the token would take them times 0.
+template <typename T, int VW, int VD>
+__device__ __forceinline__ void add_wild(const FullArgs& a, const uint64_t* at, uint32_t there,
+                                         int ahead, const float (&s)[8], const Running& run,
+                                         f32x4 (&o)[VD][VW]) {
+  const int lane = lane_now();
+  const int col = lane & 15, quad = lane >> 4;
+  Running now = run;  // its shift is not to be shared with the weights', on the way of all tokens
+  asm volatile("" : "+v"(now.m));
+  const float shift = now.shift();
+#pragma unroll 1
+  for (int k = 0; k < 32; k++) {
+    // the token's score is with the lanes of quarter k / 4 % 4
+    float mine = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) mine = 4 * (k >> 4) + (k & 3) == i ? s[i] : mine;
+    mine = __shfl(mine, col + 16 * ((k >> 2) & 3));
+    if (!((there >> k) & 1) || k > ahead) continue;
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(mine, a.scale_log2, -shift));
+    const uint64_t row = at[k] + a.skv;
+#pragma unroll
+    for (int v = 0; v < VD; v++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint64_t p = row + 2 * min(128 * v + VW * (4 * quad + r), a.d - VW);
+        uint32_t x[VW / 2];
+        if constexpr (VW == 8) {
+          const u32x4 y = load16(p);
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[j] = y[j];
+        } else {
+          const u32x2 y = load8(p);
+          x[0] = y[0];
+          x[1] = y[1];
+        }
+#pragma unroll
+        for (int j = 0; j < VW; j++) {
+          const uint16_t bits = static_cast<uint16_t>(x[j / 2] >> (16 * (j & 1)));
+          const float y = w * static_cast<float>(__builtin_bit_cast(T, bits));
+          o[v][j][r] += (bits & kWildBits<T>) == kWildBits<T> ? y : 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // few loads at once: registers are short
+      }
+  }
+}
+
+int full_attend(const FullArgs& a, int type, hipStream_t s);
 int full_weigh(const FullArgs& a, int type, int64_t max_len, int64_t max_prefix, hipStream_t s);
 
 }  // namespace evs
