@@ -6,15 +6,23 @@
 namespace evs {
 namespace {
 
-// Rows of one query joined from their parts: four elements a thread, and the parts in turn to as many
-// threads as there may be parts for; the rest of a workgroup takes further heads. Bound by latency
-// where parts are many, else by their bytes.
+// A row's parts, taken together: their maxima and totals.
+__device__ __forceinline__ void join_stats(const float* stats, int64_t at, float& top,
+                                           float& total) {
+  const float m = stats[2 * at], l = stats[2 * at + 1];
+  const float now = fmaxf(top, m);
+  const float ref = now == -INFINITY ? 0.0f : now;
+  total = total * __builtin_amdgcn_exp2f(top - ref) + l * __builtin_amdgcn_exp2f(m - ref);
+  top = now;
+}
+
+// The rows of one query, joined from their parts: four elements a thread, and the parts in turn to as
+// many threads as there may be parts for; the rest of a workgroup takes further heads.
 template <typename T>
-__global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a, int word_bits,
-                                                          int turn_bits) {
+__device__ __forceinline__ void join_rows(const FullArgs& a, int token, int first, int step,
+                                          int word_bits, int turn_bits) {
   __shared__ f32x4 s_v[kFullThreads];
   __shared__ float s_m[kFullThreads], s_l[kFullThreads];
-  const int token = blockIdx.x;
   const int s = sequence_of(a, token);
   if (s < 0) return;  // uniform
   const Rows sq = scalar_rows(sequence_rows(a, s));
@@ -22,56 +30,166 @@ __global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a, int word_b
   const int w = tid & ((1 << word_bits) - 1);
   const int turn = (tid >> word_bits) & ((1 << turn_bits) - 1);
   const int heads_at = kFullThreads >> (word_bits + turn_bits);
-  const int q_head = blockIdx.y * heads_at + (tid >> (word_bits + turn_bits));
   const int shared = a.shared.d;
-  // the tokens that the row's tile sees, and its parts
+  // the prefix, and the own part of the context that a row's tile sees
   const bool few = sq.rows <= kRowTile, alone = sq.rows > kTogether;
-  const int g = a.group.tiles > 0 || (alone && a.pre.n > 0) ? group_of(a, s) : -1;
+  const Cut& cut = few ? a.few : a.many;
+  if (!is_joined(a, cut, sq.rows, (1 << 31) - 1)) return;  // no row of it, however much it sees
+  const int g = a.pre.n > 0 ? group_of(a, s) : -1;
   const int prefix = g < 0 ? 0 : length_of(a, a.pre, g);
   const int ahead = alone ? prefix : 0;
-  const int in = min(q_head, a.q_heads - 1);
-  const int row = (token - sq.q0) * shared + in % shared;
   const int tile = few ? kRowTile : kRowTile * kFullWaves * a.row_tiles;
-  const int last = min(row / tile * tile + tile, sq.rows) - 1;
-  const int end = min(ahead + sq.len, max(ahead + sq.len - sq.nq + last / shared + 1, ahead));
-  const Cut& cut = few ? a.few : a.many;
-  const bool joined = q_head < a.q_heads && is_joined(a, cut, sq.rows, end);
-  const int before = alone || !joined ? 0 : parts_of(a.group, prefix);
-  const int parts = joined ? before + max(parts_of(cut, end), 1) : 0;
-  float top = -INFINITY, total = 0;
-  f32x4 v = {0, 0, 0, 0};
-  const int wr = min(w, a.d / 4 - 1);
+  for (int h0 = first * heads_at; h0 < a.q_heads; h0 += step * heads_at) {
+    const int q_head = h0 + (tid >> (word_bits + turn_bits));
+    const int in = min(q_head, a.q_heads - 1);
+    const int head = in / shared, row = (token - sq.q0) * shared + in - head * shared;
+    const int last = min(row / tile * tile + tile, sq.rows) - 1;
+    const int end = min(ahead + sq.len, max(ahead + sq.len - sq.nq + last / shared + 1, ahead));
+    const bool joined = q_head < a.q_heads && is_joined(a, cut, sq.rows, end);
+    const int before = alone || !joined ? 0 : parts_of(a.group, prefix);
+    const int parts = joined ? before + max(parts_of(cut, end), 1) : 0;
+    float top = -INFINITY, total = 0;
+    f32x4 v = {0, 0, 0, 0};
+    const int wr = min(w, a.d / 4 - 1);
 #pragma unroll 4
-  for (int k = turn; k < parts; k += 1 << turn_bits) {
-    const int slot = k < before ? k : a.group.splits + k - before;
-    const int64_t at = part_at(a, slot, token, in);
-    const float m = a.stats[2 * at], l = a.stats[2 * at + 1];
-    const f32x4 y = *reinterpret_cast<const f32x4*>(a.sums + at * a.d + 4 * wr);
-    const float now = fmaxf(top, m);
-    const float ref = now == -INFINITY ? 0.0f : now;
-    const float f = __builtin_amdgcn_exp2f(top - ref), h = __builtin_amdgcn_exp2f(m - ref);
-    top = now;
-    total = total * f + l * h;
-    v = v * f + y * h;
-  }
-  if (turn_bits > 0) {
-    s_v[tid] = v;
-    s_m[tid] = top;
-    s_l[tid] = total;
-    __syncthreads();
-    if (turn != 0) return;
-    for (int k = 1; k < 1 << turn_bits; k++) top = fmaxf(top, s_m[tid + (k << word_bits)]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    total = 0;
-    v = f32x4{0, 0, 0, 0};
-    for (int k = 0; k < 1 << turn_bits; k++) {
-      const int t = tid + (k << word_bits);
-      const float f = __builtin_amdgcn_exp2f(s_m[t] - ref);
-      total += s_l[t] * f;
-      v += s_v[t] * f;
+    for (int k = turn; k < parts; k += 1 << turn_bits) {
+      const bool own = few && k >= before;
+      const int64_t at = own ? few_part_at(a, k - before, s, head, row)
+                             : part_at(a, k < before ? k : a.group.splits + k - before, token, in);
+      const FullArgs::Parts& p = own ? a.few_parts : a.parts;
+      const float m = p.stats[2 * at], l = p.stats[2 * at + 1];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p.sums + at * a.d + 4 * wr);
+      const float now = fmaxf(top, m);
+      const float ref = now == -INFINITY ? 0.0f : now;
+      const float f = __builtin_amdgcn_exp2f(top - ref), h = __builtin_amdgcn_exp2f(m - ref);
+      top = now;
+      total = total * f + l * h;
+      v = v * f + y * h;
     }
+    if (turn_bits > 0) {
+      __syncthreads();  // the heads before have been read
+      s_v[tid] = v;
+      s_m[tid] = top;
+      s_l[tid] = total;
+      __syncthreads();
+      if (turn == 0) {
+        for (int k = 1; k < 1 << turn_bits; k++) top = fmaxf(top, s_m[tid + (k << word_bits)]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        total = 0;
+        v = f32x4{0, 0, 0, 0};
+        for (int k = 0; k < 1 << turn_bits; k++) {
+          const int t = tid + (k << word_bits);
+          const float f = __builtin_amdgcn_exp2f(s_m[t] - ref);
+          total += s_l[t] * f;
+          v += s_v[t] * f;
+        }
+      }
+    }
+    if (joined && turn == 0 && w < a.d / 4) finish4<T>(a, token, q_head, w, v, top, total);
   }
-  if (joined && w < a.d / 4) finish4<T>(a, token, q_head, w, v, top, total);
+}
+
+constexpr int kScored = 4 * kFullThreads;  // tokens of a workgroup
+
+// The weights of a sequence with few rows, of one KV head and 1,024 of its own tokens, from the
+// scores that the attention kept (full_weigh.hip has the formula and the other contexts). The rows'
+// references are joined from the same parts as the rows, so it need not wait for those.
+__device__ __forceinline__ void weigh_scores(const FullArgs& a, uint32_t seq, int head, int step) {
+  __shared__ float s_top[kRowTile];
+  constexpr int kAhead = 4;  // rows whose scores are on their way while the references are joined
+  const Rows sq = scalar_rows(sequence_rows(a, seq));
+  const int stop = min(sq.len, a.stored);
+  const int t0 = step * kScored;
+  if (sq.rows == 0 || sq.rows > kRowTile || t0 >= stop) return;
+  const int tid = threadIdx.x, r = tid >> 4;
+  const int past = sq.len - sq.nq;
+  const int t = t0 + 4 * tid;
+  const int in = min(t, (stop - 1) & ~3);
+  const float* scores = a.scores + few_part_at(a, 0, seq, head, 0) * a.stored + in;
+  const auto score = [&](int row) {
+    return *reinterpret_cast<const f32x4*>(
+        scores + static_cast<int64_t>(min(row, sq.rows - 1)) * a.stored);
+  };
+  f32x4 x[kAhead];
+#pragma unroll
+  for (int row = 0; row < kAhead; row++) x[row] = score(row);
+  // where the tokens' masses are; null for no token
+  const int32_t* table = a.own.tables + static_cast<int64_t>(seq) * a.own.stride;
+  float* mass[4];
+  float old[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    uint32_t n, off;
+    a.div_bs.divmod(min(in + j, stop - 1), n, off);
+    const int32_t page = table[n];
+    mass[j] = t + j >= stop || page < 0 || page >= a.num_blocks
+                  ? nullptr
+                  : a.mass + (static_cast<int64_t>(page) * a.heads + head) * a.block_size + off;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) old[j] = mass[j] == nullptr || t + j >= past ? 0.0f : *mass[j];
+  {
+    // 16 threads a row
+    const int own = max(parts_of(a.few, sq.len), 1);
+    const int g = a.pre.n > 0 ? group_of(a, seq) : -1;
+    const int before = g < 0 || a.group.tiles == 0 ? 0 : parts_of(a.group, length_of(a, a.pre, g));
+    float top = -INFINITY, total = 0;
+    if (r < sq.rows) {
+      uint32_t qi, qg;
+      a.shared.divmod(r, qi, qg);
+      for (int k = tid & 15; k < own; k += 16)
+        join_stats(a.few_parts.stats, few_part_at(a, k, seq, head, r), top, total);
+      for (int k = tid & 15; k < before; k += 16)
+        join_stats(a.parts.stats, part_at(a, k, sq.q0 + qi, head * a.shared.d + qg), top, total);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const float m = __shfl_xor(top, d), l = __shfl_xor(total, d);
+      const float now = fmaxf(top, m);
+      const float ref = now == -INFINITY ? 0.0f : now;
+      total = total * __builtin_amdgcn_exp2f(top - ref) + l * __builtin_amdgcn_exp2f(m - ref);
+      top = now;
+    }
+    if ((tid & 15) == 0)
+      s_top[r] = total == 0 ? INFINITY : top + __builtin_amdgcn_logf(total);
+  }
+  __syncthreads();
+  f32x4 sum = {0, 0, 0, 0};
+  const auto add = [&](int row, const f32x4& y) {
+    const float top = s_top[row];
+    const int sees = past + static_cast<int>(a.shared.div(row)) - t;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], a.scale_log2, -top));
+      sum[j] += sees >= j && top != INFINITY ? w : 0.0f;
+    }
+  };
+#pragma unroll
+  for (int row = 0; row < kAhead; row++)
+    if (row < sq.rows) add(row, x[row]);
+#pragma unroll 4
+  for (int row = kAhead; row < sq.rows; row++) add(row, score(row));
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if (mass[j] != nullptr) *mass[j] = old[j] + sum[j];
+}
+
+// The launch behind the attention's: the first workgroups join rows, `down` of them a query, the
+// others weigh tokens by scores, `steps` of them a sequence and head.
+template <typename T>
+__global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a, uint32_t join_items,
+                                                          FastDiv down, int word_bits,
+                                                          int turn_bits, FastDiv steps) {
+  if (blockIdx.x < join_items) {
+    uint32_t token, first;
+    down.divmod(blockIdx.x, token, first);
+    join_rows<T>(a, token, first, down.d, word_bits, turn_bits);
+  } else {
+    uint32_t rest, step, seq, head;
+    steps.divmod(blockIdx.x - join_items, rest, step);
+    a.div_heads.divmod(rest, seq, head);
+    weigh_scores(a, seq, head, step);
+  }
 }
 
 __global__ __launch_bounds__(kFullThreads) void no_weights(float* top, int64_t n) {
@@ -83,18 +201,25 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
 
 constexpr int64_t kRound = 256;  // tokens that a workgroup's waves take in turn, of few rows
-constexpr int64_t kFillRows = 1024;  // workgroups that fill the GPU, of few rows
+constexpr int64_t kFillRows = 1024;
+  // workgroups that fill the GPU, of few rows
 constexpr int64_t kFillTiles = 256;  // and of many
-constexpr int64_t kMostParts = 64;
+// Beyond that, workgroups for few rows of contexts of unlike lengths, and the tokens of one.
+constexpr int64_t kEven = 4096, kEvenChunk = 1024;
+constexpr int64_t kMostParts = 1024;
+constexpr int64_t kMostScores = int64_t{1} << 29;  // bytes of scores that a call may keep
 
 // How contexts of up to max_len tokens are cut for `tiles` row tiles that there may be: into parts
-// that make `fill` workgroups in all, of `least_chunk` tokens at least.
-Cut cut(int64_t tiles, int64_t heads, int64_t max_len, int64_t fill, int64_t least_chunk) {
+// that make `fill` workgroups in all, of `least_chunk` tokens at least, and beyond that into parts of
+// `good_chunk` tokens that make `even` of them, so that contexts of unlike lengths end together.
+Cut cut(int64_t tiles, int64_t heads, int64_t max_len, int64_t fill, int64_t least_chunk,
+        int64_t even, int64_t good_chunk) {
   Cut c{};
   if (tiles == 0) return c;
-  int64_t parts = least(least(ceil_div(fill, tiles * heads), kMostParts),
-                        ceil_div(max_len, least_chunk));
-  parts = parts < 1 ? 1 : parts;
+  const int64_t parts_fill = least(ceil_div(fill, tiles * heads), ceil_div(max_len, least_chunk));
+  const int64_t parts_even = least(ceil_div(even, tiles * heads), ceil_div(max_len, good_chunk));
+  int64_t parts = parts_fill > parts_even ? parts_fill : parts_even;
+  parts = parts < 1 ? 1 : least(parts, kMostParts);
   int64_t chunk = ceil_div(ceil_div(max_len, parts), kRound) * kRound;
   chunk = chunk < kRound ? kRound : least(chunk, (int64_t{1} << 31) - kRound);
   c.tiles = static_cast<uint32_t>(least(tiles, (int64_t{1} << 31) - 1));
@@ -122,7 +247,9 @@ struct Deal {
   Cut group, few, many;
   bool few_groups;
   int row_tiles;
-  int64_t slots, sums, stats, top, bytes;
+  int64_t slots, few_slots;  // of parts
+  int64_t few_rows, stored;
+  int64_t sums, stats, few_sums, few_stats, top, scores, bytes;
 };
 
 Deal deal(Counts n) {
@@ -136,21 +263,31 @@ Deal deal(Counts n) {
   const bool wide = n.d <= 128 && (most > kTogether || (together && rows / n.groups > kTogether));
   r.row_tiles = wide ? 2 : 1;
   const int64_t tile = kRowTile * kFullWaves * r.row_tiles;
-  if (shared <= kRowTile) r.few = cut(n.seqs, n.heads, n.max_len, kFillRows, kRound);
+  if (shared <= kRowTile) r.few = cut(n.seqs, n.heads, n.max_len, kFillRows, kRound, kEven, kEvenChunk);
   if (most > kRowTile)
     r.many = cut(least(n.seqs * ceil_div(most, tile),
                        rows / tile + least(n.seqs, rows / (kRowTile + 1))),
-                 n.heads, n.max_len + n.max_prefix, kFillTiles, 2 * kRound);
+                 n.heads, n.max_len + n.max_prefix, kFillTiles, 2 * kRound, 0, 2 * kRound);
   if (together)
-    r.group = r.few_groups ? cut(n.groups, n.heads, n.max_prefix, kFillRows, kRound)
-                           : cut(rows / tile + n.groups, n.heads, n.max_prefix, kFillTiles, kRound);
-  r.slots = r.group.splits + (r.few.splits > r.many.splits ? r.few.splits : r.many.splits);
-  if (r.slots == 1) r.slots = 0;
-  const int64_t every = n.tokens * n.q_heads;
+    r.group = r.few_groups ? cut(n.groups, n.heads, n.max_prefix, kFillRows, kRound, kEven, kEvenChunk)
+                           : cut(rows / tile + n.groups, n.heads, n.max_prefix, kFillTiles, kRound, 0, kRound);
+  // rows that are written where they go need no parts
+  r.slots = r.group.splits + (r.many.splits > 1 || r.group.splits > 0 ? r.many.splits : 0);
+  r.few_slots = r.few.splits > 1 || r.group.splits > 0 ? r.few.splits : 0;
+  r.few_rows = least(most, kRowTile);
+  const int64_t every = n.tokens * n.q_heads, few = n.seqs * n.heads * r.few_rows;
+  if (n.mass && r.few.splits > 0) {
+    r.stored = (n.max_len + 3) / 4 * 4;
+    r.scores = r.stored <= kMostScores / 4 / few ? few * r.stored * 4 : 0;
+    if (r.scores == 0) r.stored = 0;
+  }
+  const auto on16 = [](int64_t x) { return (x + 15) / 16 * 16; };
   r.sums = r.slots * every * n.d * 4;
-  r.stats = r.slots * every * 8;
-  r.top = n.mass ? every * 4 : 0;
-  r.bytes = (r.sums + r.stats + r.top + 15) / 16 * 16;
+  r.stats = on16(r.slots * every * 8);
+  r.few_sums = r.few_slots * few * n.d * 4;
+  r.few_stats = on16((r.stored > 0 ? r.few.splits : r.few_slots) * few * 8);
+  r.top = n.mass ? on16(every * 4) : 0;
+  r.bytes = r.sums + r.stats + r.few_sums + r.few_stats + r.top + r.scores;
   return r;
 }
 
@@ -286,34 +423,59 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
     a.pre.n = static_cast<int32_t>(groups);
     a.group_starts = group_starts;
   }
+  a.few_rows = static_cast<int32_t>(deal.few_rows);
   char* at = static_cast<char*>(workspace);
-  a.sums = reinterpret_cast<float*>(at);
-  a.stats = reinterpret_cast<float*>(at + deal.sums);
+  const auto take = [&](int64_t bytes) {
+    float* p = reinterpret_cast<float*>(at);
+    at += bytes;
+    return p;
+  };
+  a.parts.sums = take(deal.sums);
+  a.parts.stats = take(deal.stats);
+  a.few_parts.sums = take(deal.few_sums);
+  a.few_parts.stats = take(deal.few_stats);
   if (mass != nullptr) {
     a.mass = mass;
-    a.top = reinterpret_cast<float*>(at + deal.sums + deal.stats);
+    a.top = take(deal.top);
+    if (deal.stored > 0) a.scores = take(deal.scores);
+    a.stored = static_cast<int32_t>(deal.stored);
   }
   const hipStream_t s = evs::as_stream(stream);
-  if (mass != nullptr && q_starts != nullptr) {
-    // queries that no sequence names have no weights
+  if (mass != nullptr && q_starts != nullptr && deal.group.tiles > 0) {
+    // queries of a group that no sequence names have no weights
     const int64_t rows = tokens * q_heads;
     evs::no_weights<<<static_cast<uint32_t>((rows + 255) / 256), evs::kFullThreads, 0, s>>>(a.top,
                                                                                           rows);
     EVS_LAUNCHED(who);
   }
   if (const int rc = evs::full_attend(a, type, s)) return rc;
-  if (deal.slots > 0) {
-    int word_bits = 0, turn_bits = 0;
-    while ((4 << word_bits) < head_dim) word_bits++;
-    while (word_bits + turn_bits < 8 && (4 << turn_bits) < deal.slots) turn_bits++;
-    const int64_t heads_at = evs::kFullThreads >> (word_bits + turn_bits);
-    const dim3 grid(static_cast<uint32_t>(tokens),
-                    static_cast<uint32_t>((q_heads + heads_at - 1) / heads_at));
+  // workgroups that join rows, enough of them for each query to fill the GPU, and that weigh tokens
+  const int64_t slots = deal.group.splits + (deal.few.splits > deal.many.splits ? deal.few.splits
+                                                                                : deal.many.splits);
+  int word_bits = 0, turn_bits = 0;
+  while ((4 << word_bits) < head_dim) word_bits++;
+  while (word_bits + turn_bits < 8 && (4 << turn_bits) < slots) turn_bits++;
+  const int64_t heads_at = evs::kFullThreads >> (word_bits + turn_bits);
+  int64_t down = (q_heads + heads_at - 1) / heads_at;
+  if (down > 4096 / tokens + 1) down = 4096 / tokens + 1;
+  const int64_t joins = deal.slots + deal.few_slots > 0 ? tokens * down : 0;
+  const int64_t steps = deal.stored > 0 ? (deal.stored + evs::kScored - 1) / evs::kScored : 0;
+  const int64_t items = joins + seqs * heads * steps;
+  if (items > 0) {
+    const evs::FastDiv by_down(static_cast<uint32_t>(down));
+    const evs::FastDiv by_steps(static_cast<uint32_t>(steps > 0 ? steps : 1));
+    const uint32_t grid = static_cast<uint32_t>(items), first = static_cast<uint32_t>(joins);
     if (type == EVS_BF16)
-      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a, word_bits, turn_bits);
+      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a, first, by_down, word_bits,
+                                                               turn_bits, by_steps);
     else
-      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a, word_bits, turn_bits);
+      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a, first, by_down, word_bits,
+                                                                 turn_bits, by_steps);
     EVS_LAUNCHED(who);
   }
-  return mass == nullptr ? EVS_OK : evs::full_weigh(a, type, n.max_len, n.max_prefix, s);
+  // what is left to weigh: prefixes, contexts of many rows, tokens without a score
+  const bool left = deal.group.tiles > 0 || deal.many.tiles > 0 ||
+                    deal.stored < evs::room(0, width, block_size);
+  return mass == nullptr || !left ? EVS_OK
+                                  : evs::full_weigh(a, type, n.max_len, n.max_prefix, s);
 }

@@ -68,11 +68,19 @@ struct FullArgs {
   // how prefixes are cut for their groups' rows, own tokens for few rows, and contexts for many
   Cut group, few, many;
   bool few_groups;  // a group has at most kRowTile rows
-  // parts: sums [slots, tokens, q_heads, d], maxima and totals [slots, tokens, q_heads, 2]; the
-  // prefix's parts first
-  float* sums;
-  float* stats;
+  // Parts: sums [slots, rows, d], maxima and totals [slots, rows, 2]. `parts`: a row is a query and
+  // head, and a slot a part of its group's prefix or, behind those, of a context for many rows.
+  // `few_parts`: the slots are parts of own tokens for few rows, [seqs, heads, few_rows].
+  struct Parts {
+    float* sums;
+    float* stats;
+  } parts, few_parts;
+  int32_t few_rows;
   int32_t row_tiles;  // of 16 rows, that a wave has of a tile of many
+  // scores of few rows with their own tokens, for the weights: [seqs, heads, few_rows, stored], of
+  // the first `stored` tokens; or null
+  float* scores;
+  int32_t stored;
   float* mass;  // [num_blocks, heads, block_size], or null
 };
 
@@ -281,7 +289,7 @@ __device__ __forceinline__ void load_query(const FullArgs& a, const char* p, int
 
 // Eight scores of this lane's row to weights, as an operand.
 template <typename T>
-__device__ __forceinline__ u32x4 full_weights(const float (&s)[8], float scale_log2, Running& r) {
+__device__ __forceinline__ u32x4 full_weights(const float* s, float scale_log2, Running& r) {
   const float shift = r.shift();
   u32x4 p;
 #pragma unroll
@@ -299,6 +307,19 @@ __device__ __forceinline__ u32x4 full_weights(const float (&s)[8], float scale_l
 __device__ __forceinline__ int64_t part_at(const FullArgs& a, int32_t slot, int32_t token,
                                            int32_t q_head) {
   return (static_cast<int64_t>(slot) * a.tokens + token) * a.q_heads + q_head;
+}
+__device__ __forceinline__ int64_t few_part_at(const FullArgs& a, int32_t slot, int32_t seq,
+                                               int32_t head, int32_t row) {
+  return ((static_cast<int64_t>(slot) * a.seqs + seq) * a.heads + head) * a.few_rows + row;
+}
+
+__device__ __forceinline__ void keep4(const FullArgs::Parts& p, int d, int64_t at, int w, f32x4 v,
+                                      float top, float total) {
+  *reinterpret_cast<f32x4*>(p.sums + at * d + 4 * w) = v;
+  if (w == 0) {
+    p.stats[2 * at] = top;
+    p.stats[2 * at + 1] = total;
+  }
 }
 
 // Four elements of an output row, 4 w on, from the sums, their reference and the weights' total.
@@ -319,29 +340,13 @@ __device__ __forceinline__ void finish4(const FullArgs& a, int32_t token, int32_
   }
 }
 
-// Four sums of a row: to its part if it is joined, else to the output.
-template <typename T>
-__device__ __forceinline__ void put4(const FullArgs& a, bool joined, int32_t slot, int32_t token,
-                                     int32_t q_head, int w, f32x4 v, float top, float total) {
-  if (joined) {
-    const int64_t at = part_at(a, slot, token, q_head);
-    *reinterpret_cast<f32x4*>(a.sums + at * a.d + 4 * w) = v;
-    if (w == 0) {
-      a.stats[2 * at] = top;
-      a.stats[2 * at + 1] = total;
-    }
-  } else {
-    finish4<T>(a, token, q_head, w, v, top, total);
-  }
-}
-
 // The products of the values that are no finite numbers among 32 tokens, whose rows are at `at` and
 // whose scores for this lane's row are `s`: the row's elements get them if it sees the token, of
 // which it sees those up to `ahead`. Such values are kept out of the other products, where a row
 // ahead of the token would take them times 0.
 template <typename T, int VW, int VD>
 __device__ __forceinline__ void add_wild(const FullArgs& a, const uint64_t* at, uint32_t there,
-                                         int ahead, const float (&s)[8], const Running& run,
+                                         int ahead, const float* s, const Running& run,
                                          f32x4 (&o)[VD][VW]) {
   const int lane = lane_now();
   const int col = lane & 15, quad = lane >> 4;

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(kFullThreads, NG > 4 ? 1 : 2) void attend_full(Full
 
 // A launch without many rows.
 template <typename T, int NG, bool kWhole>
-__global__ __launch_bounds__(kFullThreads, NG > 4 ? 1 : NG == 4 && !kWhole ? 2 : 3) void attend_full_rows(FullArgs a,
+__global__ __launch_bounds__(kFullThreads, NG > 4 ? 1 : 2) void attend_full_rows(FullArgs a,
                                                                                  Items n) {
   __shared__ RowsLds<NG> lds;
   rows_part<T, NG, kWhole, 1>(a, lds, blockIdx.x, n.row_prefixes);

@@ -117,6 +117,11 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
     for (int j = 0; j < VW; j++) o[v][j] = f32x4{0, 0, 0, 0};
   Running run[1];
 
+  // (token t's score with this lane's row goes to scores[t])
+  float* scores = prefix || a.scores == nullptr
+                      ? nullptr
+                      : a.scores + few_part_at(a, 0, who, head, min(col, last_row)) * a.stored;
+
   const int first = begin + 64 * wave;
   if (first < stop) {
     const int step = 64 * kFullWaves;
@@ -172,7 +177,8 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
         for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][k & 3];
         const bool whole = t + 32 <= all_see && there == 0xFFFFFFFFu;
         bool wild = false;
-        if (!whole) {
+        if (__builtin_expect(!whole, false)) {
+          asm volatile("");  // a branch: most tokens need none of it
           const int ahead[1] = {sees - t - 4 * quad};
           mask<1>(s, ahead, there >> (4 * quad));
           // rows of no tokens are to be numbers, whatever the pages hold: their weight is 0; so
@@ -223,6 +229,15 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
             o[v][2 * k + 1] = mma<T>(odd, w, o[v][2 * k + 1]);
           }
         x.fetch_values(a, next, lane);
+        // behind the loads: waiting for those is not to wait for this
+        if (scores != nullptr && col < sq.rows) {
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const uint32_t at = static_cast<uint32_t>(t) + 16 * g + 4 * quad;
+            if (at < static_cast<uint32_t>(a.stored))
+              *reinterpret_cast<f32x4*>(scores + at) = acc[g];
+          }
+        }
       }
       ok = ok_next;
     }
@@ -246,8 +261,7 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
   }
   __syncthreads();
   const int words = a.d / 4;
-  const int slot = prefix ? split : a.group.splits + split;
-  const bool joined = prefix || is_joined(a, cut, sq.rows, end);
+  const bool joined = prefix || is_joined(a, a.few, sq.rows, end);
   for (int x = threadIdx.x; x < sq.rows * words; x += kFullThreads) {
     const int r = x / words, w = x - r * words;
     float top = -INFINITY;
@@ -264,7 +278,19 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
     }
     uint32_t i, g;
     a.shared.divmod(r, i, g);
-    put4<T>(a, joined, slot, sq.q0 + i, head * a.shared.d + g, w, v, top, total);
+    const int token = sq.q0 + i, q_head = head * a.shared.d + g;
+    if (prefix)
+      keep4(a.parts, a.d, part_at(a, split, token, q_head), w, v, top, total);
+    else if (joined)
+      keep4(a.few_parts, a.d, few_part_at(a, split, who, head, r), w, v, top, total);
+    else
+      finish4<T>(a, token, q_head, w, v, top, total);
+    if (!joined && a.scores != nullptr && w == 0) {
+      // the weights' references
+      float* stats = a.few_parts.stats + 2 * few_part_at(a, split, who, head, r);
+      stats[0] = top;
+      stats[1] = total;
+    }
   }
 }
 

@@ -264,61 +264,81 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
       const int t0 = begin + i * kTokens;
       if (t0 >= wave_stop) continue;
       const bool wild = __builtin_amdgcn_ballot_w64(lds.wild[i & 3][lane & (kFullWaves - 1)] != 0) != 0;
+      f32x4 acc[kSubs][2][kTiles];
 #pragma unroll
-      for (int sub = 0; sub < kSubs; sub++) {
-        const int t = t0 + 32 * sub;
-        if (t >= wave_stop) continue;
-        f32x4 acc[2][kTiles];
+      for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
-          for (int n = 0; n < kTiles; n++) acc[g][n] = f32x4{0, 0, 0, 0};
+          for (int n = 0; n < kTiles; n++) acc[sub][g][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
         for (int c = 0; c < NG; c++)
 #pragma unroll
           for (int g = 0; g < 2; g++) {
             const u32x4 k = lds.key[i & 1][sub][g][c][lane];
 #pragma unroll
-            for (int n = 0; n < kTiles; n++) acc[g][n] = mma<T>(k, q[n][c], acc[g][n]);
+            for (int n = 0; n < kTiles; n++) acc[sub][g][n] = mma<T>(k, q[n][c], acc[sub][g][n]);
           }
-        float s[kTiles][8];
+      float s[kTiles][8 * kSubs];
+#pragma unroll
+      for (int n = 0; n < kTiles; n++)
+#pragma unroll
+        for (int k = 0; k < 8 * kSubs; k++) s[n][k] = acc[k >> 3][(k >> 2) & 1][n][k & 3];
+      uint32_t ok[kSubs], all = 0xFFFFFFFFu;
+#pragma unroll
+      for (int sub = 0; sub < kSubs; sub++) {
+        ok[sub] = __builtin_amdgcn_readfirstlane(lds.ok[i & 3][sub]);
+        all &= ok[sub];
+      }
+      if (__builtin_expect(t0 + kTokens > all_see || all != 0xFFFFFFFFu, false)) {
+        asm volatile("");  // a branch: most stages need none of it
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++)
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const int at = 16 * (k >> 2) + 4 * quad + (k & 3);
+            const bool in = (ok[sub] >> at) & 1;
+#pragma unroll
+            for (int n = 0; n < kTiles; n++)
+              s[n][8 * sub + k] =
+                  in && t0 + 32 * sub + at <= sees[n] ? s[n][8 * sub + k] : -INFINITY;
+          }
+      }
+      float fade[kTiles];
+      if (grow<kTiles>(s, a.scale_log2, run, fade)) {
 #pragma unroll
         for (int n = 0; n < kTiles; n++)
 #pragma unroll
-          for (int k = 0; k < 8; k++) s[n][k] = acc[k >> 2][n][k & 3];
-        const uint32_t ok = __builtin_amdgcn_readfirstlane(lds.ok[i & 3][sub]);
-        if (t + 32 > all_see || ok != 0xFFFFFFFFu) {
-          int ahead[kTiles];
+          for (int v = 0; v < VD; v++)
 #pragma unroll
-          for (int n = 0; n < kTiles; n++) ahead[n] = sees[n] - t - 4 * quad;
-          mask<kTiles>(s, ahead, ok >> (4 * quad));
-        }
-        float fade[kTiles];
-        if (grow<kTiles>(s, a.scale_log2, run, fade)) {
+            for (int j = 0; j < VW; j++) o[n][v][j] *= fade[n];
+      }
+      if (__builtin_expect(wild, false)) {
+#pragma unroll
+        for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
           for (int n = 0; n < kTiles; n++)
+            add_wild<T, VW, VD>(a, lds.at[i & 3] + 32 * sub, ok[sub], sees[n] - t0 - 32 * sub,
+                                &s[n][8 * sub], run[n], o[n]);
+      }
+      u32x4 p[kSubs][kTiles];
 #pragma unroll
-            for (int v = 0; v < VD; v++)
+      for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
-              for (int j = 0; j < VW; j++) o[n][v][j] *= fade[n];
-        }
-        if (__builtin_expect(wild, false)) {
+        for (int n = 0; n < kTiles; n++)
+          p[sub][n] = full_weights<T>(&s[n][8 * sub], a.scale_log2, run[n]);
 #pragma unroll
-          for (int n = 0; n < kTiles; n++)
-            add_wild<T, VW, VD>(a, lds.at[i & 3] + 32 * sub, ok, sees[n] - t, s[n], run[n], o[n]);
-        }
-        u32x4 p[kTiles];
-#pragma unroll
-        for (int n = 0; n < kTiles; n++) p[n] = full_weights<T>(s[n], a.scale_log2, run[n]);
+      for (int sub = 0; sub < kSubs; sub++)
 #pragma unroll
         for (int v = 0; v < VD; v++)
 #pragma unroll
           for (int j = 0; j < VW; j++) {
             const u32x4 x = lds.value[i & 1][sub][v][j][lane];
 #pragma unroll
-            for (int n = 0; n < kTiles; n++) o[n][v][j] = mma<T>(x, p[n], o[n][v][j]);
+            for (int n = 0; n < kTiles; n++) o[n][v][j] = mma<T>(x, p[sub][n], o[n][v][j]);
           }
-      }
     }
   }
 
@@ -339,10 +359,13 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
 #pragma unroll
         for (int j = 0; j < VW; j += 4) {
           const int e = 128 * v + VW * (4 * quad + r) + j;
-          if (e < a.d)
-            put4<T>(a, joined, slot, sq.q0 + i, head * a.shared.d + g, e / 4,
-                    f32x4{o[n][v][j][r], o[n][v][j + 1][r], o[n][v][j + 2][r], o[n][v][j + 3][r]},
-                    run[n].m, l);
+          if (e >= a.d) continue;
+          const f32x4 x = {o[n][v][j][r], o[n][v][j + 1][r], o[n][v][j + 2][r], o[n][v][j + 3][r]};
+          const int token = sq.q0 + i, q_head = head * a.shared.d + g;
+          if (joined)
+            keep4(a.parts, a.d, part_at(a, slot, token, q_head), e / 4, x, run[n].m, l);
+          else
+            finish4<T>(a, token, q_head, e / 4, x, run[n].m, l);
         }
   }
 }

@@ -9,13 +9,21 @@
 namespace evs {
 namespace {
 
-constexpr int kStep = 32 * kFullWaves;  // tokens of a workgroup
+// Tokens of a wave, whose keys stay in registers while the rows pass.
+template <int NG>
+constexpr int kKept = NG > 4 ? 32 : 64;
+constexpr int kManyRows = 64;  // rows from which a workgroup's waves share them, not the tokens
 
-// One workgroup: every so-many-th 128 tokens of a context and KV head, 32 of them a wave, whose keys
-// stay in registers while the rows pass.
+// One workgroup: the tokens of a context and KV head from kKept times `at` on, at every so-many-th
+// place. The rows of a context with many are dealt to the waves in tiles of 16, and a token's sums
+// joined in LDS; else each wave has tokens of its own. Bound by the exponentials where rows are many
+// (for 16 rows and 64 tokens 256 cycles of them, and 256 of matrix instructions, which run beside
+// them), else by reading K.
 template <typename T, int NG>
 __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t prefix_items,
                                                            FastDiv prefix_steps, FastDiv own_steps) {
+  constexpr int kG = kKept<NG> / 16;
+  __shared__ float s_sum[kFullWaves][kKept<NG>];
   const bool prefix = blockIdx.x < prefix_items;
   const Contexts& c = prefix ? a.pre : a.own;
   const FastDiv& steps = prefix ? prefix_steps : own_steps;
@@ -23,18 +31,24 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
   a.div_heads.divmod(prefix ? blockIdx.x : blockIdx.x - prefix_items, rest, head);
   steps.divmod(rest, who, at);
   const Rows sq = scalar_rows(prefix ? group_rows(a, who) : sequence_rows(a, who));
+  if (sq.rows == 0) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int past = prefix ? sq.len : sq.len - sq.nq;
   const int32_t* table = c.tables + static_cast<int64_t>(who) * c.stride;
   const uint64_t base = reinterpret_cast<uint64_t>(a.base) + head * a.sh;
-  for (int64_t first = static_cast<int64_t>(at) * kStep + 32 * wave; first < sq.len;
-       first += static_cast<int64_t>(steps.d) * kStep) {
+  const bool by_rows = sq.rows >= kManyRows;
+  const int64_t span = by_rows ? kKept<NG> : kKept<NG> * kFullWaves;
+  const int row_step = by_rows ? kRowTile * kFullWaves : kRowTile;
+  // tokens that the scores kept have been weighed by
+  const int64_t done = !prefix && sq.rows <= kRowTile ? a.stored : 0;
+  for (int64_t first = done + at * span + (by_rows ? 0 : kKept<NG> * wave); first < sq.len;
+       first += steps.d * span) {
     const int t = static_cast<int>(first);
-    u32x4 k[2][NG];
+    u32x4 k[kG][NG];
 #pragma unroll
-    for (int g = 0; g < 2; g++) {
+    for (int g = 0; g < kG; g++) {
       uint32_t n, off;
       a.div_bs.divmod(min(static_cast<uint32_t>(t) + 16 * g + col,
                           static_cast<uint32_t>(sq.len) - 1),
@@ -51,42 +65,86 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
         for (int j = 0; j < 4; j++) k[g][i][j] = in ? x[j] : 0;
       }
     }
-    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    float sum[kG][4];
+#pragma unroll
+    for (int g = 0; g < kG; g++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) sum[g][r] = 0;
     const int from = max(t - past, 0) * static_cast<int>(a.shared.d);  // the first row that sees t
-    for (int row0 = from / kRowTile * kRowTile; row0 < sq.rows; row0 += kRowTile) {
-      const bool in = row0 + col < sq.rows;
+    const int row_first = from / kRowTile * kRowTile + (by_rows ? kRowTile * wave : 0);
+    u32x4 q[NG];
+    float top;
+    int sees;
+    const auto load = [&](int row0, u32x4 (&to)[NG], float& reference, int& last) {
       uint32_t qi, qg;
       a.shared.divmod(min(row0 + col, sq.rows - 1), qi, qg);
       const int64_t token = sq.q0 + qi;
       const int q_head = head * a.shared.d + qg;
-      u32x4 q[NG];
-      load_query<NG>(a, a.q + token * a.q_token + q_head * a.q_head, quad, q);
-      const float top = in ? a.top[token * a.q_heads + q_head] : INFINITY;
-      f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      load_query<NG>(a, a.q + token * a.q_token + q_head * a.q_head, quad, to);
+      reference = row0 + col < sq.rows ? a.top[token * a.q_heads + q_head] : INFINITY;
+      last = past + static_cast<int>(qi) - t - 4 * quad;
+    };
+    if (row_first < sq.rows) load(row_first, q, top, sees);
+    for (int row0 = row_first; row0 < sq.rows; row0 += row_step) {
+      // the next rows are on their way
+      u32x4 q_next[NG];
+      float top_next;
+      int sees_next;
+      load(row0 + row_step, q_next, top_next, sees_next);
+      f32x4 acc[kG];
+#pragma unroll
+      for (int g = 0; g < kG; g++) acc[g] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < NG; i++)
 #pragma unroll
-        for (int g = 0; g < 2; g++) acc[g] = mma<T>(k[g][i], q[i], acc[g]);
-      const int sees = past + static_cast<int>(qi) - t - 4 * quad;
+        for (int g = 0; g < kG; g++) acc[g] = mma<T>(k[g][i], q[i], acc[g]);
+      // (rows that see nothing have no weights, whatever their scores)
+      const bool all = sees + 4 * quad >= kKept<NG> - 1 && top != INFINITY;
+      if (__builtin_amdgcn_ballot_w64(!all) == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float w = __builtin_amdgcn_exp2f(
-            __builtin_fmaf(acc[j >> 2][j & 3], a.scale_log2, -top));
-        // (rows that see nothing have no weights, whatever their scores)
-        sum[j] += sees >= 16 * (j >> 2) + (j & 3) && top != INFINITY ? w : 0.0f;
+        for (int g = 0; g < kG; g++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            sum[g][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
+      } else {
+#pragma unroll
+        for (int g = 0; g < kG; g++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float w =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
+            sum[g][r] += sees >= 16 * g + r && top != INFINITY ? w : 0.0f;
+          }
       }
+#pragma unroll
+      for (int i = 0; i < NG; i++) q[i] = q_next[i];
+      top = top_next;
+      sees = sees_next;
     }
+    // over the rows of a tile, which are the lanes of a quarter
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+    for (int g = 0; g < kG; g++)
 #pragma unroll
-      for (int d = 1; d < 16; d <<= 1) sum[j] += __shfl_xor(sum[j], d);
-    if (col < 8) {
-      // lane `col` of a quarter has token 16 (col / 4) + 4 quad + col % 4
-      float mine = sum[0];
+      for (int r = 0; r < 4; r++)
 #pragma unroll
-      for (int j = 1; j < 8; j++) mine = col == j ? sum[j] : mine;
-      const uint32_t own = static_cast<uint32_t>(t) + 16 * (col >> 2) + 4 * quad + (col & 3);
+        for (int d = 1; d < 16; d <<= 1) sum[g][r] += __shfl_xor(sum[g][r], d);
+    if (by_rows) __syncthreads();  // the sums before have been read
+    if (col == 0) {
+#pragma unroll
+      for (int g = 0; g < kG; g++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s_sum[wave][16 * g + 4 * quad + r] = sum[g][r];
+    }
+    if (by_rows)
+      __syncthreads();
+    else
+      __builtin_amdgcn_wave_barrier();
+    if (lane < kKept<NG> && (!by_rows || wave == 0)) {
+      const uint32_t own = static_cast<uint32_t>(t) + lane;
       if (own < static_cast<uint32_t>(sq.len)) {
+        float mine = s_sum[wave][lane];
+        if (by_rows)
+          for (int w = 1; w < kFullWaves; w++) mine += s_sum[w][lane];
         uint32_t n, off;
         a.div_bs.divmod(own, n, off);
         const int32_t page = table[n];
@@ -115,10 +173,11 @@ void launch(const FullArgs& a, uint32_t items, uint32_t prefix_items, FastDiv pr
     weigh_full<T, 8><<<items, kFullThreads, 0, s>>>(a, prefix_items, prefix_steps, own_steps);
 }
 
-// Workgroups that take the steps of a context in turn: one a step, fewer where there are very many.
-uint32_t steps_of(int64_t max_len, int64_t contexts, int64_t heads) {
-  const int64_t steps = (max_len + kStep - 1) / kStep;
-  const int64_t most = (int64_t{1} << 20) / (contexts * heads) + 1;
+// Workgroups that take the places of a context in turn: one a place, fewer where there are very many.
+uint32_t steps_of(const FullArgs& a, int64_t max_len, int64_t contexts, int64_t rows) {
+  const int64_t kept = (a.d > 128 ? 32 : 64) * (rows >= kManyRows ? 1 : kFullWaves);
+  const int64_t steps = (max_len + kept - 1) / kept;
+  const int64_t most = (int64_t{1} << 20) / (contexts * a.heads) + 1;
   const int64_t n = steps < most ? steps : most;
   return static_cast<uint32_t>(n < 1 ? 1 : n);
 }
@@ -126,8 +185,11 @@ uint32_t steps_of(int64_t max_len, int64_t contexts, int64_t heads) {
 }  // namespace
 
 int full_weigh(const FullArgs& a, int type, int64_t max_len, int64_t max_prefix, hipStream_t s) {
-  const FastDiv own(steps_of(max_len, a.own.n, a.heads));
-  const FastDiv pre(a.pre.n > 0 ? steps_of(max_prefix, a.pre.n, a.heads) : 1);
+  const int64_t shared = a.shared.d, most = a.max_q * shared;  // rows of a sequence
+  // (where the scores of few rows are kept only tokens past them are left, which there rarely are)
+  const bool mostly = a.stored > 0 && most <= kRowTile;
+  const FastDiv own(mostly ? 1 : steps_of(a, max_len, a.own.n, most));
+  const FastDiv pre(a.pre.n > 0 ? steps_of(a, max_prefix, a.pre.n, a.tokens * shared) : 1);
   const int64_t prefix_items = static_cast<int64_t>(a.pre.n) * pre.d * a.heads;
   const int64_t items = prefix_items + static_cast<int64_t>(a.own.n) * own.d * a.heads;
   EVS_REQUIRE(items < (int64_t{1} << 23), "evs_attend: too many sequences and heads to weigh");

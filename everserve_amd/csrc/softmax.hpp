@@ -88,10 +88,10 @@ __device__ __forceinline__ void mask(float (&s)[kTiles][8], const int (&ahead)[k
   }
 }
 
-// Whether eight new scores of each of this lane's rows (masked ones -infinity) take some row's
-// maximum too far past its reference: then all sums so far must be multiplied by `fade`.
-template <int kTiles>
-__device__ __forceinline__ bool grow(const float (&s)[kTiles][8], float scale_log2,
+// Whether new scores of each of this lane's rows (masked ones -infinity) take some row's maximum too
+// far past its reference: then all sums so far must be multiplied by `fade`.
+template <int kTiles, int kScores>
+__device__ __forceinline__ bool grow(const float (&s)[kTiles][kScores], float scale_log2,
                                      Running (&r)[kTiles], float (&fade)[kTiles]) {
   float top[kTiles];
   bool far = false;
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool grow(const float (&s)[kTiles][8], float scale_lo
   for (int n = 0; n < kTiles; n++) {
     float x = s[n][0];
 #pragma unroll
-    for (int k = 1; k < 8; k++) x = fmaxf(x, s[n][k]);
+    for (int k = 1; k < kScores; k++) x = fmaxf(x, s[n][k]);
     top[n] = x * scale_log2;
     far |= top[n] > r[n].m + kSlack;
   }
