@@ -16,32 +16,44 @@ __device__ __forceinline__ void join_stats(const float* stats, int64_t at, float
   top = now;
 }
 
-// The rows of one query, joined from their parts: four elements a thread, and the parts in turn to as
-// many threads as there may be parts for; the rest of a workgroup takes further heads.
+// How the rows of a query are dealt to workgroups for the join: 2^words threads have four elements
+// each of a row (or of a piece of it: `pieces` of them), 2^turns threads take the parts in turn, and
+// the rest of a workgroup takes further heads; `down` workgroups take a query's heads and pieces.
+struct JoinShape {
+  int words, turns;
+  FastDiv pieces, down;
+};
+
+// The rows of one query, joined from their parts.
 template <typename T>
-__device__ __forceinline__ void join_rows(const FullArgs& a, int token, int first, int step,
-                                          int word_bits, int turn_bits) {
+__device__ __forceinline__ void join_rows(const FullArgs& a, int token, int first,
+                                          const JoinShape& shape) {
   __shared__ f32x4 s_v[kFullThreads];
   __shared__ float s_m[kFullThreads], s_l[kFullThreads];
   const int s = sequence_of(a, token);
   if (s < 0) return;  // uniform
   const Rows sq = scalar_rows(sequence_rows(a, s));
-  const int tid = threadIdx.x;
-  const int w = tid & ((1 << word_bits) - 1);
-  const int turn = (tid >> word_bits) & ((1 << turn_bits) - 1);
-  const int heads_at = kFullThreads >> (word_bits + turn_bits);
   const int shared = a.shared.d;
   // the prefix, and the own part of the context that a row's tile sees
   const bool few = sq.rows <= kRowTile, alone = sq.rows > kTogether;
   const Cut& cut = few ? a.few : a.many;
-  if (!is_joined(a, cut, sq.rows, (1 << 31) - 1)) return;  // no row of it, however much it sees
+  if (!is_joined(a, cut, sq.rows, (1u << 31) - 1)) return;  // no row of it, however much it sees
   const int g = a.pre.n > 0 ? group_of(a, s) : -1;
   const int prefix = g < 0 ? 0 : length_of(a, a.pre, g);
   const int ahead = alone ? prefix : 0;
   const int tile = few ? kRowTile : kRowTile * kFullWaves * a.row_tiles;
-  for (int h0 = first * heads_at; h0 < a.q_heads; h0 += step * heads_at) {
-    const int q_head = h0 + (tid >> (word_bits + turn_bits));
+  const int tid = threadIdx.x;
+  const int mine = shape.words + shape.turns;
+  const int heads_at = kFullThreads >> mine;
+  const int turn = (tid >> shape.words) & ((1 << shape.turns) - 1);
+  const int items = (a.q_heads + heads_at - 1) / heads_at * shape.pieces.d;
+  for (int item = first; item < items; item += shape.down.d) {
+    uint32_t at, piece;
+    shape.pieces.divmod(item, at, piece);
+    const int q_head = at * heads_at + (tid >> mine);
     const int in = min(q_head, a.q_heads - 1);
+    const int w = (piece << shape.words) + (tid & ((1 << shape.words) - 1));
+    const int wr = min(w, a.d / 4 - 1);
     const int head = in / shared, row = (token - sq.q0) * shared + in - head * shared;
     const int last = min(row / tile * tile + tile, sq.rows) - 1;
     const int end = min(ahead + sq.len, max(ahead + sq.len - sq.nq + last / shared + 1, ahead));
@@ -50,15 +62,14 @@ __device__ __forceinline__ void join_rows(const FullArgs& a, int token, int firs
     const int parts = joined ? before + max(parts_of(cut, end), 1) : 0;
     float top = -INFINITY, total = 0;
     f32x4 v = {0, 0, 0, 0};
-    const int wr = min(w, a.d / 4 - 1);
-#pragma unroll 4
-    for (int k = turn; k < parts; k += 1 << turn_bits) {
+#pragma unroll 8
+    for (int k = turn; k < parts; k += 1 << shape.turns) {
       const bool own = few && k >= before;
-      const int64_t at = own ? few_part_at(a, k - before, s, head, row)
-                             : part_at(a, k < before ? k : a.group.splits + k - before, token, in);
+      const int64_t i = own ? few_part_at(a, k - before, s, head, row)
+                            : part_at(a, k < before ? k : a.group.splits + k - before, token, in);
       const FullArgs::Parts& p = own ? a.few_parts : a.parts;
-      const float m = p.stats[2 * at], l = p.stats[2 * at + 1];
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p.sums + at * a.d + 4 * wr);
+      const float m = p.stats[2 * i], l = p.stats[2 * i + 1];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p.sums + i * a.d + 4 * wr);
       const float now = fmaxf(top, m);
       const float ref = now == -INFINITY ? 0.0f : now;
       const float f = __builtin_amdgcn_exp2f(top - ref), h = __builtin_amdgcn_exp2f(m - ref);
@@ -66,19 +77,20 @@ __device__ __forceinline__ void join_rows(const FullArgs& a, int token, int firs
       total = total * f + l * h;
       v = v * f + y * h;
     }
-    if (turn_bits > 0) {
+    if (shape.turns > 0) {
       __syncthreads();  // the heads before have been read
       s_v[tid] = v;
       s_m[tid] = top;
       s_l[tid] = total;
       __syncthreads();
       if (turn == 0) {
-        for (int k = 1; k < 1 << turn_bits; k++) top = fmaxf(top, s_m[tid + (k << word_bits)]);
+        for (int k = 1; k < 1 << shape.turns; k++)
+          top = fmaxf(top, s_m[tid + (k << shape.words)]);
         const float ref = top == -INFINITY ? 0.0f : top;
         total = 0;
         v = f32x4{0, 0, 0, 0};
-        for (int k = 0; k < 1 << turn_bits; k++) {
-          const int t = tid + (k << word_bits);
+        for (int k = 0; k < 1 << shape.turns; k++) {
+          const int t = tid + (k << shape.words);
           const float f = __builtin_amdgcn_exp2f(s_m[t] - ref);
           total += s_l[t] * f;
           v += s_v[t] * f;
@@ -174,16 +186,15 @@ __device__ __forceinline__ void weigh_scores(const FullArgs& a, uint32_t seq, in
     if (mass[j] != nullptr) *mass[j] = old[j] + sum[j];
 }
 
-// The launch behind the attention's: the first workgroups join rows, `down` of them a query, the
-// others weigh tokens by scores, `steps` of them a sequence and head.
+// The launch behind the attention's: the first workgroups join rows, the others weigh tokens by
+// scores, `steps` of them a sequence and head.
 template <typename T>
 __global__ __launch_bounds__(kFullThreads) void join_full(FullArgs a, uint32_t join_items,
-                                                          FastDiv down, int word_bits,
-                                                          int turn_bits, FastDiv steps) {
+                                                          JoinShape shape, FastDiv steps) {
   if (blockIdx.x < join_items) {
     uint32_t token, first;
-    down.divmod(blockIdx.x, token, first);
-    join_rows<T>(a, token, first, down.d, word_bits, turn_bits);
+    shape.down.divmod(blockIdx.x, token, first);
+    join_rows<T>(a, token, first, shape);
   } else {
     uint32_t rest, step, seq, head;
     steps.divmod(blockIdx.x - join_items, rest, step);
@@ -268,9 +279,13 @@ Deal deal(Counts n) {
     r.many = cut(least(n.seqs * ceil_div(most, tile),
                        rows / tile + least(n.seqs, rows / (kRowTile + 1))),
                  n.heads, n.max_len + n.max_prefix, kFillTiles, 2 * kRound, 0, 2 * kRound);
+  // A prefix's parts are long ones where there is much to do beside them: 64 sequences of up to 1,024
+  // tokens behind one prompt of 8 Ki 62 us for 65 (kFillTiles workgroups for it), 16 of 2,001 behind
+  // 131 Ki, where they are all there is, 40 us for 48.
+  const bool busy = static_cast<int64_t>(r.few.tiles) * r.few.splits * n.heads >= 2 * kFillTiles;
   if (together)
     r.group = r.few_groups ? cut(n.groups, n.heads, n.max_prefix, kFillRows, kRound, kEven, kEvenChunk)
-                           : cut(rows / tile + n.groups, n.heads, n.max_prefix, kFillTiles, kRound, 0, kRound);
+                           : cut((rows + n.groups * (tile - 1)) / tile, n.heads, n.max_prefix, busy ? kFillTiles / 2 : kFillTiles, kRound, 0, kRound);
   // rows that are written where they go need no parts
   r.slots = r.group.splits + (r.many.splits > 1 || r.group.splits > 0 ? r.many.splits : 0);
   r.few_slots = r.few.splits > 1 || r.group.splits > 0 ? r.few.splits : 0;
@@ -452,25 +467,31 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   // workgroups that join rows, enough of them for each query to fill the GPU, and that weigh tokens
   const int64_t slots = deal.group.splits + (deal.few.splits > deal.many.splits ? deal.few.splits
                                                                                 : deal.many.splits);
-  int word_bits = 0, turn_bits = 0;
-  while ((4 << word_bits) < head_dim) word_bits++;
-  while (word_bits + turn_bits < 8 && (4 << turn_bits) < slots) turn_bits++;
-  const int64_t heads_at = evs::kFullThreads >> (word_bits + turn_bits);
-  int64_t down = (q_heads + heads_at - 1) / heads_at;
-  if (down > 4096 / tokens + 1) down = 4096 / tokens + 1;
+  evs::JoinShape shape{};
+  int64_t pieces = 1, down = 1;
+  {
+    // four elements a thread; a row in pieces of 32 elements where there are many parts of few rows
+    while ((4 << shape.words) < head_dim) shape.words++;
+    if (slots >= 32 && tokens * q_heads < 2048)
+      while (shape.words > 3) shape.words--;
+    pieces = (head_dim / 4 + (1 << shape.words) - 1) >> shape.words;
+    while (shape.words + shape.turns < 8 && (8 << shape.turns) < slots) shape.turns++;
+    const int64_t heads_at = evs::kFullThreads >> (shape.words + shape.turns);
+    down = (q_heads + heads_at - 1) / heads_at * pieces;
+    if (down > 4096 / tokens + 1) down = 4096 / tokens + 1;
+  }
+  shape.pieces = evs::FastDiv(static_cast<uint32_t>(pieces));
+  shape.down = evs::FastDiv(static_cast<uint32_t>(down));
   const int64_t joins = deal.slots + deal.few_slots > 0 ? tokens * down : 0;
   const int64_t steps = deal.stored > 0 ? (deal.stored + evs::kScored - 1) / evs::kScored : 0;
   const int64_t items = joins + seqs * heads * steps;
   if (items > 0) {
-    const evs::FastDiv by_down(static_cast<uint32_t>(down));
     const evs::FastDiv by_steps(static_cast<uint32_t>(steps > 0 ? steps : 1));
     const uint32_t grid = static_cast<uint32_t>(items), first = static_cast<uint32_t>(joins);
     if (type == EVS_BF16)
-      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a, first, by_down, word_bits,
-                                                               turn_bits, by_steps);
+      evs::join_full<__bf16><<<grid, evs::kFullThreads, 0, s>>>(a, first, shape, by_steps);
     else
-      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a, first, by_down, word_bits,
-                                                                 turn_bits, by_steps);
+      evs::join_full<_Float16><<<grid, evs::kFullThreads, 0, s>>>(a, first, shape, by_steps);
     EVS_LAUNCHED(who);
   }
   // what is left to weigh: prefixes, contexts of many rows, tokens without a score

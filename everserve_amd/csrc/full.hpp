@@ -146,41 +146,34 @@ __device__ __forceinline__ bool is_joined(const FullArgs& a, const Cut& c, int32
   return parts_of(c, end) > 1 || (rows <= kTogether && a.group.tiles > 0);
 }
 
-// The one of `n` with place `at` on a line on which each has count(i) places, found by the whole
-// workgroup of kFullThreads; false past the line's end.
-template <typename Count>
-__device__ __forceinline__ bool find_place(uint32_t n, uint32_t at, Count count, uint32_t& who,
-                                           uint32_t& place) {
-  __shared__ uint32_t s_wave[kFullWaves];
-  __shared__ uint32_t s_who, s_place;
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t before = 0;
-  for (uint32_t i0 = 0; i0 < n; i0 += kFullThreads) {
-    const uint32_t i = i0 + tid;
-    const uint32_t mine = i < n ? count(i) : 0;
+// The one of `n` with place `at` on a line on which the rows rows_of(i) have count(rows) places, found
+// by each wave for itself, without a wait for others; false past the line's end.
+template <typename RowsOf, typename Count>
+__device__ __forceinline__ bool find_rows(uint32_t n, uint32_t at, RowsOf rows_of, Count count,
+                                          uint32_t& who, uint32_t& place, Rows& found) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+    Rows r{};
+    if (i0 + lane < n) r = rows_of(i0 + lane);
+    const uint32_t mine = i0 + lane < n ? count(r) : 0;
     uint32_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t up = __shfl_up(sum, d);
       if (lane >= static_cast<uint32_t>(d)) sum += up;
     }
-    if (lane == 63) s_wave[wave] = sum;
-    __syncthreads();
-    uint32_t from = before + sum - mine;
-    for (uint32_t k = 0; k < kFullWaves; k++) {
-      if (k < wave) from += s_wave[k];
-      before += s_wave[k];
-    }
-    if (at >= from && at - from < mine) {
-      s_who = i;
-      s_place = at - from;
-    }
-    __syncthreads();
-    if (at < before) {
-      who = __builtin_amdgcn_readfirstlane(s_who);
-      place = __builtin_amdgcn_readfirstlane(s_place);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(at < sum);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      who = i0 + l;
+      place = at - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+      found.q0 = __builtin_amdgcn_readlane(r.q0, l);
+      found.nq = __builtin_amdgcn_readlane(r.nq, l);
+      found.rows = __builtin_amdgcn_readlane(r.rows, l);
+      found.len = __builtin_amdgcn_readlane(r.len, l);
       return true;
     }
+    at -= __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
 }

@@ -89,25 +89,39 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
   a.div_heads.divmod(prefix ? item : item - prefix_items, rest, head);
   split = rest / cut.tiles;
   who = rest - split * cut.tiles;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t* table = c.tables + static_cast<int64_t>(who) * c.stride;
+  const int begin = split * cut.chunk;
+  const int first = begin + 64 * wave;
+  constexpr int step = 64 * kFullWaves;
+  // The first pages are read ahead of the length, which they do not wait for; so tokens are kept
+  // within the table, and what lies past the length is no token. (Without a sign: past the last
+  // pair a token may pass 2^31.)
+  const uint32_t room = static_cast<uint32_t>(
+      min(static_cast<int64_t>(c.width) * a.block_size, (int64_t{1} << 31) - 1));
+  const auto token_of = [&](int p) {
+    return static_cast<uint32_t>(first) + static_cast<uint32_t>(p * step + lane);
+  };
+  const auto page_of = [&](int p) {
+    return room == 0 ? -1 : table[a.div_bs.div(min(token_of(p), room - 1))];
+  };
+  int32_t page = page_of(0), page_next = page_of(1);
   const Rows sq = scalar_rows(prefix ? group_rows(a, who) : sequence_rows(a, who));
   if (sq.rows == 0 || sq.rows > kRowTile) return;
   const int last_row = sq.rows - 1;
   // own tokens are seen up to the query's own, a prefix by every row
   const int past = prefix ? sq.len : sq.len - sq.nq;
   const int end = prefix ? sq.len : min(sq.len, past + sq.nq);
-  const int begin = split * cut.chunk;
   const int stop =
       static_cast<int>(split) + 1 == cut.splits ? end : min(end, begin + cut.chunk);
   if (begin >= stop && (prefix || split > 0)) return;
 
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   uint32_t qi, qg;
   a.shared.divmod(min(col, last_row), qi, qg);
   const int sees = past + static_cast<int>(qi);  // this lane's row: the tokens up to this one
   const int all_see = min(stop, past + 1);
-  const int32_t* table = c.tables + static_cast<int64_t>(who) * c.stride;
   const uint64_t base = reinterpret_cast<uint64_t>(a.base) + head * a.sh;
 
   f32x4 o[VD][VW];
@@ -122,27 +136,17 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
                       ? nullptr
                       : a.scores + few_part_at(a, 0, who, head, min(col, last_row)) * a.stored;
 
-  const int first = begin + 64 * wave;
   if (first < stop) {
-    const int step = 64 * kFullWaves;
     const int pairs = (stop - first + step - 1) / step;
-    // (without a sign: past the last pair it may pass 2^31)
-    const auto token_of = [&](int p) {
-      return static_cast<uint32_t>(first) + static_cast<uint32_t>(p * step + lane);
-    };
-    const auto page_of = [&](int p) {
-      return table[a.div_bs.div(min(token_of(p), static_cast<uint32_t>(stop) - 1))];
-    };
     // the addresses of a pair's tokens, and which of them are tokens
     const auto locate = [&](int p, int32_t page) {
       const uint32_t t = token_of(p);
       uint32_t n, off;
-      a.div_bs.divmod(min(t, static_cast<uint32_t>(stop) - 1), n, off);
+      a.div_bs.divmod(min(t, room - 1), n, off);
       const bool ok = t < static_cast<uint32_t>(stop) && page >= 0 && page < a.num_blocks;
       lds.at[wave][p & 1][lane] = base + (ok ? page * a.sb + static_cast<int64_t>(off) * a.so : 0);
       return __builtin_amdgcn_ballot_w64(ok);
     };
-    int32_t page = page_of(0), page_next = page_of(1);
     u32x4 q[NG];
     load_query<NG>(a, a.q + (sq.q0 + qi) * a.q_token + (head * a.shared.d + qg) * a.q_head, quad,
                    q);

@@ -130,21 +130,26 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
   // Workgroups go to the 8 XCDs in turn: all row tiles of a head and part to one, whose rows then
   // stay in its L2.
   const uint32_t unit = at / (8 * cut.tiles) * 8 + (at & 7);
-  const uint32_t place = (at >> 3) % cut.tiles;
+  // (the last first: of a sequence's tiles they see the most tokens)
+  const uint32_t place = cut.tiles - 1 - (at >> 3) % cut.tiles;
   uint32_t head, split, who, tile;
   a.div_heads.divmod(unit, split, head);
   if (static_cast<int>(split) >= cut.splits) return;
-  const auto tiles_of = [&](uint32_t i) -> uint32_t {
-    const Rows r = prefix ? group_rows(a, i) : sequence_rows(a, i);
+  Rows sq;
+  const auto tiles_of = [&](const Rows& r) -> uint32_t {
     return prefix || r.rows > kRowTile ? (r.rows + kRows - 1) / kRows : 0;
   };
-  if (!find_place(prefix ? a.pre.n : a.own.n, place, tiles_of, who, tile)) return;
-  const Rows sq = scalar_rows(prefix ? group_rows(a, who) : sequence_rows(a, who));
+  if (prefix ? !find_rows(a.pre.n, place, [&](uint32_t i) { return group_rows(a, i); }, tiles_of,
+                          who, tile, sq)
+             : !find_rows(a.own.n, place, [&](uint32_t i) { return sequence_rows(a, i); }, tiles_of,
+                          who, tile, sq))
+    return;
   const int row0 = tile * kRows, last_row = min(row0 + kRows, sq.rows) - 1;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  int ahead_len = 0;  // tokens of a prefix ahead of the own ones
+  bool needed = true;  // this wave's rows
+  int ahead_len = 0;   // tokens of a prefix ahead of the own ones
   const int32_t* ahead_table = nullptr;
   if (prefix) {
     if (a.starts != nullptr && a.max_q * static_cast<int>(a.shared.d) > kTogether) {
@@ -153,12 +158,17 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
       const int to = sq.q0 + static_cast<int>(a.shared.div(last_row));
       const int s0 = min(max(a.group_starts[who], 0), a.seqs);
       const int s1 = min(max(a.group_starts[who + 1], s0), a.seqs);
-      bool any = false;
+      const int wave_from = sq.q0 + static_cast<int>(a.shared.div(row0 + 16 * kTiles * wave));
+      const int wave_to = sq.q0 + static_cast<int>(a.shared.div(row0 + 16 * kTiles * (wave + 1) - 1));
+      bool any = false, mine = false;
       for (int s = s0 + lane; s < s1; s += 64) {
         const Rows r = sequence_rows(a, s);
-        any |= r.rows > 0 && r.rows <= kTogether && r.q0 <= to && r.q0 + r.nq > from;
+        const bool with = r.rows > 0 && r.rows <= kTogether;
+        any |= with && r.q0 <= to && r.q0 + r.nq > from;
+        mine |= with && r.q0 <= wave_to && r.q0 + r.nq > wave_from;
       }
       if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+      needed = __builtin_amdgcn_ballot_w64(mine) != 0;
     }
   } else if (sq.rows > kTogether) {
     const int g = group_of(a, who);
@@ -182,7 +192,7 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
 
   // this wave's rows, and the tokens that some and all of them see
   const int wave0 = row0 + 16 * kTiles * wave;
-  const bool any_row = wave0 <= last_row;
+  const bool any_row = needed && wave0 <= last_row;
   const int wave_stop =
       any_row ? min(stop, seen_by(min(wave0 + 16 * kTiles - 1, last_row))) : 0;
   const int all_see = any_row ? min(stop, seen_by(wave0)) : 0;
@@ -240,11 +250,11 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
 #pragma unroll
     for (int k = 0; k < 3; k++) pages[k] = page_of(k);
     int32_t page = page_of(3);
-#pragma unroll
-    for (int k = 0; k < 3; k++) locate(k, pages[k]);
     u32x4 q[kTiles][NG];
 #pragma unroll
     for (int n = 0; n < kTiles; n++) load_query<NG>(a, qp[n], quad, q[n]);
+#pragma unroll
+    for (int k = 0; k < 3; k++) locate(k, pages[k]);
     __syncthreads();
     const auto tame = [&](int stage) { return begin + (stage + 1) * kTokens > tile_see; };
     Staged<T, NG, kWhole> rows;
@@ -349,7 +359,7 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
   for (int n = 0; n < kTiles; n++) {
     const float l = across_rows_sum(run[n].l);
     const int row = wave0 + 16 * n + col;
-    if (row > last_row) continue;
+    if (!any_row || row > last_row) continue;
     uint32_t i, g;
     a.shared.divmod(row, i, g);
 #pragma unroll
