@@ -5,23 +5,19 @@
 namespace evs {
 namespace {
 
-constexpr int kChooseThreads = 512;
-constexpr int kChooseWaves = kChooseThreads / 64;
-constexpr int kRun = 8;                          // tokens a thread takes side by side
-constexpr int kSpan = kChooseThreads * kRun;     // and a workgroup at once
-constexpr uint32_t kHeld = 8192;                 // keys kept in LDS
+constexpr int kRun = 8;           // tokens a thread takes side by side
+constexpr uint32_t kHeld = 8192;  // masses kept in LDS
 constexpr uint32_t kBins = 2048;
+constexpr int kPasses = 3;
+constexpr int kShift[kPasses] = {21, 10, 0};
 
 struct ChooseArgs {
-  float* mass;  // [layers, num_blocks, heads, block_size]
+  const float* mass;  // [layers, num_blocks, heads, block_size]
   int32_t num_blocks, block_size;
   FastDiv div_bs, div_heads, div_seqs;
   const int32_t* tables;
   int64_t table_stride;
   int32_t width;
-  const int32_t* new_tables;
-  int64_t new_stride;
-  int32_t new_width;
   const int32_t* lens;
   int32_t seqs, heads, budget, recent;
   int32_t* lens_out;
@@ -42,38 +38,56 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Inclusive sums of two counts (16 bits each) over the workgroup, in order of its threads; `total`
-// gets all of it.
-__device__ __forceinline__ uint32_t scan2(uint32_t mine, uint32_t (&s_wave)[kChooseWaves],
-                                          uint32_t& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t sum = mine;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// The bin, from the largest down, in which `left` keys are reached, by a wave; `left` gets how many of
+// the bin's keys are wanted.
+__device__ __forceinline__ uint32_t reached(const uint32_t* bins, uint32_t& left) {
+  const uint32_t lane = threadIdx.x & 63;
+  constexpr uint32_t kOf = kBins / 64;  // a lane's bins
+  const auto scan = [&](uint32_t x) {
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t up = __shfl_up(sum, d);
-    if (lane >= d) sum += up;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t up = __shfl_up(x, d);
+      if (lane >= static_cast<uint32_t>(d)) x += up;
+    }
+    return x;
+  };
+  uint32_t mine = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kOf; i += 4) {
+    const uint4 x = *reinterpret_cast<const uint4*>(bins + kBins - (lane + 1) * kOf + i);
+    mine += x.x + x.y + x.z + x.w;
   }
-  __syncthreads();  // the sums before have been read
-  if (lane == 63) s_wave[wave] = sum;
-  __syncthreads();
-  total = 0;
-  for (int k = 0; k < kChooseWaves; k++) {
-    if (k < wave) sum += s_wave[k];
-    total += s_wave[k];
-  }
-  return sum;
+  const uint32_t sum = scan(mine);
+  const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum >= left) | (1ull << 63));
+  left -= __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l);
+  // that lane's bins, one a lane
+  const uint32_t top = kBins - 1 - l * kOf;
+  const uint32_t one = lane < kOf ? bins[top - lane] : 0;
+  const uint32_t in = scan(one);
+  const int k = __builtin_ctzll(__builtin_amdgcn_ballot_w64(in >= left) | (1ull << 63));
+  left -= __builtin_amdgcn_readlane(in, k) - __builtin_amdgcn_readlane(one, k);
+  return top - k;
 }
 
 // One workgroup a layer, sequence and KV head. Of n tokens the `recent` last stay and the others
 // with the largest masses, `budget` in all, of equal ones the first: the least mass that stays is
 // found from the top bits down (11, 11 and 10 of them, by counting), then the tokens are taken in
-// order.
-__global__ __launch_bounds__(kChooseThreads) void choose(ChooseArgs a) {
-  __shared__ uint32_t s_key[kHeld];
-  __shared__ uint32_t s_bin[kBins];
-  __shared__ uint32_t s_wave[kChooseWaves];
-  __shared__ uint32_t s_found, s_left;
-  const uint32_t tid = threadIdx.x;
+// order. kVector: masses are read four at a time, as a page's lie.
+//
+// Bound by latency: its waits for memory, for LDS and for the other waves. Contexts that do not fit
+// LDS are read from their pages four times, eight reads a thread under way at once.
+template <bool kVector, int kThreads>
+__global__ __launch_bounds__(kThreads) void choose(ChooseArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kAt = kVector ? 4 : 1;  // masses of a read
+  constexpr int kAhead = 8;             // reads under way
+  constexpr uint32_t kSpan = kThreads * kRun;
+  __shared__ alignas(16) float s_mass[kHeld];
+  __shared__ alignas(16) uint32_t s_bin[kPasses][kBins];
+  __shared__ uint32_t s_wave[2][kWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t head, rest, seq, layer;
   a.div_heads.divmod(blockIdx.x, rest, head);
   a.div_seqs.divmod(rest, layer, seq);
@@ -83,111 +97,136 @@ __global__ __launch_bounds__(kChooseThreads) void choose(ChooseArgs a) {
   if (layer == 0 && head == 0 && tid == 0) a.lens_out[seq] = stay;
   if (a.budget == 0) return;
   const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
-  const int32_t* new_table = a.new_tables + static_cast<int64_t>(seq) * a.new_stride;
-  float* mass = a.mass + (static_cast<int64_t>(layer) * a.num_blocks * a.heads + head) *
-                             a.block_size;
+  const float* mass = a.mass + (static_cast<int64_t>(layer) * a.num_blocks * a.heads + head) *
+                                   a.block_size;
   const int64_t page_stride = static_cast<int64_t>(a.heads) * a.block_size;
   int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
-  const auto place = [&](const int32_t* pages, uint32_t t) -> float* {
-    uint32_t p, off;
-    a.div_bs.divmod(t, p, off);
-    const int32_t page = pages[p];
-    return page < 0 || page >= a.num_blocks ? nullptr : mass + page * page_stride + off;
-  };
-  const auto read_key = [&](uint32_t t) -> uint32_t {
-    const float* m = place(table, t);
-    return m == nullptr ? 0u : key_of(*m);
-  };
-  // token t stays as the j-th
-  const auto keep = [&](uint32_t t, uint32_t j) {
-    kept[j] = static_cast<int32_t>(t);
-    const float* from = place(table, t);
-    uint32_t p, off;
-    a.div_bs.divmod(j, p, off);
-    if (from == nullptr || static_cast<int32_t>(p) >= a.new_width) return;
-    float* to = place(new_table, j);
-    if (to != nullptr) *to = *from;
-  };
-  for (int32_t j = stay + tid; j < a.budget; j += kChooseThreads) kept[j] = -1;
-  if (n <= a.budget) {
-    for (int32_t t = tid; t < n; t += kChooseThreads) keep(t, t);
-    return;
-  }
   const uint32_t newest = static_cast<uint32_t>(n - min(a.recent, stay));  // the first of them
   const uint32_t want = stay - (n - newest);  // others that stay
+  for (int32_t j = stay + tid; j < a.budget; j += kThreads) kept[j] = -1;
+  if (n <= a.budget || want == 0) {
+    const uint32_t from = n <= a.budget ? 0 : newest;
+    for (uint32_t j = tid; j < static_cast<uint32_t>(stay); j += kThreads) kept[j] = from + j;
+    return;
+  }
   const bool in_lds = newest <= kHeld;
-  if (in_lds)
-    for (uint32_t t = tid; t < newest; t += kChooseThreads) s_key[t] = read_key(t);
+  // A mass on a page outside the cache is less than all others; its key is 0, which no other has.
+  struct Read {
+    f32x4 x;
+    bool there;
+    __device__ uint32_t key(int i) const { return there ? key_of(x[i]) : 0; }
+  };
+  // kAhead reads, `step` tokens apart, from t on; past the last token they are of no page
+  const auto read = [&](uint32_t t, uint32_t step, Read (&r)[kAhead]) {
+    int64_t at[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      uint32_t p, off;
+      a.div_bs.divmod(min(t + u * step, newest - 1), p, off);
+      const int32_t page = table[p];
+      r[u].there = page >= 0 && page < a.num_blocks;
+      at[u] = r[u].there ? page * page_stride + (kVector ? off & ~3u : off) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; u++) {
+      if constexpr (kVector)
+        r[u].x = *reinterpret_cast<const f32x4*>(mass + at[u]);
+      else
+        r[u].x[0] = mass[at[u]];
+    }
+  };
+  for (uint32_t b = 4 * tid; b < kPasses * kBins; b += 4 * kThreads)
+    *reinterpret_cast<uint4*>(&s_bin[0][b]) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
   // the least key that stays, and how many of its tokens do
   uint32_t least = 0, left = want;
 #pragma unroll
-  for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const uint32_t bins = pass == 2 ? 1024 : 2048;
-    for (uint32_t b = tid; b < bins; b += kChooseThreads) s_bin[b] = 0;
-    __syncthreads();
-    const uint32_t above = pass == 0 ? 0 : ~uint32_t{0} << (pass == 1 ? 21 : 10);
-    for (uint32_t t = tid; t < newest; t += kChooseThreads) {
-      const uint32_t k = in_lds ? s_key[t] : read_key(t);
-      if (((k ^ least) & above) == 0) atomicAdd(&s_bin[(k >> shift) & (bins - 1)], 1u);
+  for (int pass = 0; pass < kPasses; pass++) {
+    const auto count = [&](uint32_t k) {
+      const uint32_t above = pass == 0 ? 0 : ~uint32_t{0} << kShift[pass - 1];
+      const bool in = ((k ^ least) & above) == 0;
+      const uint32_t bin = (k >> kShift[pass]) & (pass == 2 ? 1023 : 2047);
+      // lanes with the first lane's bin are counted at once: masses are often alike
+      const uint32_t same = __builtin_amdgcn_readfirstlane(bin);
+      const unsigned long long all = __builtin_amdgcn_ballot_w64(in && bin == same);
+      if (in && bin != same)
+        atomicAdd(&s_bin[pass][bin], 1u);
+      else if (in && lane == static_cast<uint32_t>(__builtin_ctzll(all)))
+        atomicAdd(&s_bin[pass][bin], static_cast<uint32_t>(__builtin_popcountll(all)));
+    };
+    if (pass == 0 || !in_lds) {
+      for (uint32_t t0 = kAt * tid; t0 < newest; t0 += kAt * kThreads * kAhead) {
+        Read r[kAhead];
+        read(t0, kAt * kThreads, r);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const uint32_t t = t0 + u * kAt * kThreads;
+#pragma unroll
+          for (int i = 0; i < kAt; i++)
+            if (t + i < newest) {
+              const uint32_t k = r[u].key(i);
+              if (pass == 0 && in_lds) s_mass[t + i] = __builtin_bit_cast(float, k);
+              count(k);
+            }
+        }
+      }
+    } else {
+      for (uint32_t t = tid; t < newest; t += kThreads)
+        count(__builtin_bit_cast(uint32_t, s_mass[t]));
     }
     __syncthreads();
-    // from the largest bin down, the one in which `left` tokens are reached
-    uint32_t mine = 0;
-    const uint32_t per = bins / kChooseThreads;
-    const uint32_t top = bins - 1 - tid * per;  // this thread's first bin
-    for (uint32_t i = 0; i < per; i++) mine += s_bin[top - i];
-    const int lane = tid & 63, wave = tid >> 6;
+    least |= reached(s_bin[pass], left) << kShift[pass];
+  }
+  uint32_t taken = 0, equal = 0;  // tokens above the least key, and with it, so far
+  for (uint32_t t0 = 0, round = 0; t0 < newest; t0 += kSpan, round ^= 1) {
+    const uint32_t t = t0 + kRun * tid;
+    uint32_t k[kRun];
+    if (in_lds) {
+#pragma unroll
+      for (int i = 0; i < kRun; i++)
+        k[i] = t + i < newest ? __builtin_bit_cast(uint32_t, s_mass[t + i]) : 0;
+    } else {
+      Read r[kAhead];
+      read(t, kAt, r);
+#pragma unroll
+      for (int i = 0; i < kRun; i++) k[i] = t + i < newest ? r[i / kAt].key(i % kAt) : 0;
+    }
+    uint32_t over = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+      over |= (t + i < newest && k[i] > least ? 1u : 0u) << i;
+      same |= (t + i < newest && k[i] == least ? 1u : 0u) << i;
+    }
+    // both counts of the threads before this one, 16 bits each
+    const uint32_t mine = __popc(over) | __popc(same) << 16;
     uint32_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t up = __shfl_up(sum, d);
-      if (lane >= d) sum += up;
+      if (lane >= static_cast<uint32_t>(d)) sum += up;
     }
-    if (lane == 63) s_wave[wave] = sum;
+    if (lane == 63) s_wave[round][wave] = sum;
     __syncthreads();
-    for (int k = 0; k < wave; k++) sum += s_wave[k];
-    uint32_t before = sum - mine;
-    if (before < left && left <= sum) {
-      uint32_t b = top;
-      while (before + s_bin[b] < left) before += s_bin[b--];
-      s_found = b;
-      s_left = left - before;
-    }
-    __syncthreads();
-    if (left > 0) {
-      least |= s_found << shift;
-      left = s_left;
-    }
-  }
-  // (with no others to keep, none of them is above the largest key)
-  if (want == 0) least = 0xFFFFFFFFu;
-  uint32_t taken = 0, equal = 0;
-  for (uint32_t t0 = 0; t0 < newest && taken < want; t0 += kSpan) {
-    const uint32_t t = t0 + kRun * tid;
-    uint32_t over = 0, same = 0;
-#pragma unroll
-    for (int i = 0; i < kRun; i++) {
-      if (t + i >= newest) break;
-      const uint32_t k = in_lds ? s_key[t + i] : read_key(t + i);
-      over |= (k > least ? 1u : 0u) << i;
-      same |= (k == least ? 1u : 0u) << i;
+    uint32_t total = 0;
+    sum -= mine;
+    for (uint32_t w = 0; w < kWaves; w++) {
+      if (w < wave) sum += s_wave[round][w];
+      total += s_wave[round][w];
     }
     // of the equal ones the first `left`
-    uint32_t total;
-    uint32_t rank = equal + scan2(__popc(same), s_wave, total) - __popc(same);
-    equal += total;
+    uint32_t rank = equal + (sum >> 16);
+    uint32_t j = taken + (sum & 0xFFFF) + min(rank, left);
 #pragma unroll
-    for (int i = 0; i < kRun; i++)
-      if ((same >> i) & 1) over |= (rank++ < left ? 1u : 0u) << i;
-    uint32_t j = taken + scan2(__popc(over), s_wave, total) - __popc(over);
-    taken += total;
-#pragma unroll
-    for (int i = 0; i < kRun; i++)
-      if ((over >> i) & 1) keep(t + i, j++);
+    for (int i = 0; i < kRun; i++) {
+      const bool stays = (over >> i & 1) || ((same >> i & 1) && rank < left);
+      rank += same >> i & 1;
+      if (stays) kept[j++] = t + i;
+    }
+    taken += total & 0xFFFF;
+    equal += total >> 16;
   }
-  for (uint32_t t = newest + tid; t < static_cast<uint32_t>(n); t += kChooseThreads)
-    keep(t, want + (t - newest));
+  for (uint32_t t = newest + tid; t < static_cast<uint32_t>(n); t += kThreads)
+    kept[want + (t - newest)] = t;
 }
 
 // ---------------------------------------------------------------- the rows
@@ -198,6 +237,7 @@ constexpr uint32_t kPairs = 64;  // (token, head) pairs of a workgroup
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct MoveArgs {
+  float* mass;
   const int64_t* layer_ptrs;
   int64_t sb, so, sh, skv;  // in bytes
   int32_t num_blocks, block_size;
@@ -221,7 +261,8 @@ struct MovedWord {
 
 // The kept rows of a layer and sequence, in tiles of `tokens` new slots and a few heads: their
 // places are worked out once into LDS, then words follow one another along a half-row, the K and
-// then the V of a pair, pair by pair. A row on a page that the cache does not have is not moved.
+// then the V of a pair, pair by pair, and its mass. A row on a page that the cache does not have is
+// not moved.
 template <typename T>
 __global__ __launch_bounds__(kMoveThreads) void move_kept(MoveArgs a) {
   __shared__ int64_t s_from[kPairs], s_to[kPairs];
@@ -254,6 +295,9 @@ __global__ __launch_bounds__(kMoveThreads) void move_kept(MoveArgs a) {
       if (page >= 0 && page < a.num_blocks && into >= 0 && into < a.num_blocks) {
         from = page * a.sb + static_cast<int64_t>(off) * a.so + head * a.sh;
         to = into * a.sb + static_cast<int64_t>(noff) * a.so + head * a.sh;
+        float* mass = a.mass + static_cast<int64_t>(layer) * a.num_blocks * a.heads * a.block_size;
+        mass[(static_cast<int64_t>(into) * a.heads + head) * a.block_size + noff] =
+            mass[(static_cast<int64_t>(page) * a.heads + head) * a.block_size + off];
       }
     }
     s_from[threadIdx.x] = from;
@@ -332,7 +376,7 @@ extern "C" int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t 
                    (layer_ptrs != nullptr && mass != nullptr && kept != nullptr)),
               "%s: null argument", who);
   const int64_t items = num_layers * seqs * num_heads;
-  EVS_REQUIRE(items < most / evs::kChooseThreads, "%s: %lld layers, sequences and heads", who,
+  EVS_REQUIRE(items < most / 1024, "%s: %lld layers, sequences and heads", who,
               static_cast<long long>(items));
   const hipStream_t s = evs::as_stream(stream);
   evs::ChooseArgs c{};
@@ -345,9 +389,6 @@ extern "C" int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t 
   c.tables = tables;
   c.table_stride = table_stride;
   c.width = static_cast<int32_t>(width);
-  c.new_tables = new_tables;
-  c.new_stride = new_stride;
-  c.new_width = static_cast<int32_t>(new_width);
   c.lens = lens;
   c.seqs = static_cast<int32_t>(seqs);
   c.heads = static_cast<int32_t>(num_heads);
@@ -376,7 +417,8 @@ extern "C" int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t 
   m.table_stride = table_stride;
   m.new_tables = new_tables;
   m.new_stride = new_stride;
-  m.new_width = c.new_width;
+  m.new_width = static_cast<int32_t>(new_width);
+  m.mass = mass;
   m.lens_out = lens_out;
   m.kept = kept;
   m.seqs = c.seqs;
@@ -391,16 +433,29 @@ extern "C" int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t 
   const int64_t tiles = seqs * m.token_tiles.d * m.head_tiles.d;
   EVS_REQUIRE(tiles < most / evs::kMoveThreads, "%s: %lld tiles of rows", who,
               static_cast<long long>(tiles));
-  evs::choose<<<static_cast<uint32_t>(items), evs::kChooseThreads, 0, s>>>(c);
+  // (a page's masses start on 16 bytes if their number is a multiple of four)
+  const bool vector = block_size % 4 == 0 && reinterpret_cast<uintptr_t>(mass) % 16 == 0;
+  const uint32_t grid = static_cast<uint32_t>(items);
+  // twice the threads where a workgroup may have more tokens than LDS holds
+  if (width * block_size > evs::kHeld) {
+    if (vector)
+      evs::choose<true, 1024><<<grid, 1024, 0, s>>>(c);
+    else
+      evs::choose<false, 1024><<<grid, 1024, 0, s>>>(c);
+  } else if (vector) {
+    evs::choose<true, 512><<<grid, 512, 0, s>>>(c);
+  } else {
+    evs::choose<false, 512><<<grid, 512, 0, s>>>(c);
+  }
   EVS_LAUNCHED(who);
   if (budget == 0) return EVS_OK;
-  const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>(num_layers));
+  const dim3 move(static_cast<uint32_t>(tiles), static_cast<uint32_t>(num_layers));
   switch (word) {
-    case 16: evs::move_kept<evs::u32x4><<<grid, evs::kMoveThreads, 0, s>>>(m); break;
-    case 8: evs::move_kept<uint64_t><<<grid, evs::kMoveThreads, 0, s>>>(m); break;
-    case 4: evs::move_kept<uint32_t><<<grid, evs::kMoveThreads, 0, s>>>(m); break;
-    case 2: evs::move_kept<uint16_t><<<grid, evs::kMoveThreads, 0, s>>>(m); break;
-    default: evs::move_kept<uint8_t><<<grid, evs::kMoveThreads, 0, s>>>(m); break;
+    case 16: evs::move_kept<evs::u32x4><<<move, evs::kMoveThreads, 0, s>>>(m); break;
+    case 8: evs::move_kept<uint64_t><<<move, evs::kMoveThreads, 0, s>>>(m); break;
+    case 4: evs::move_kept<uint32_t><<<move, evs::kMoveThreads, 0, s>>>(m); break;
+    case 2: evs::move_kept<uint16_t><<<move, evs::kMoveThreads, 0, s>>>(m); break;
+    default: evs::move_kept<uint8_t><<<move, evs::kMoveThreads, 0, s>>>(m); break;
   }
   EVS_LAUNCHED(who);
   return EVS_OK;
