@@ -146,6 +146,10 @@ __global__ __launch_bounds__(kThreads) void choose(ChooseArgs a) {
       const uint32_t above = pass == 0 ? 0 : ~uint32_t{0} << kShift[pass - 1];
       const bool in = ((k ^ least) & above) == 0;
       const uint32_t bin = (k >> kShift[pass]) & (pass == 2 ? 1023 : 2047);
+      if (pass > 0) {  // few are left
+        if (in) atomicAdd(&s_bin[pass][bin], 1u);
+        return;
+      }
       // lanes with the first lane's bin are counted at once: masses are often alike
       const uint32_t same = __builtin_amdgcn_readfirstlane(bin);
       const unsigned long long all = __builtin_amdgcn_ballot_w64(in && bin == same);

@@ -14,6 +14,8 @@ struct TilesLds {
   static constexpr int VD = Fetched<NG>::VD, VW = Fetched<NG>::VW;
   static constexpr int kSubs = kStageTokens<NG> / 32;
   // operands as the lanes read them, of this stage and the next
+  // (K's chunks, of which a row has 4 NG, with a row's place among its 16 turned by the chunk's, so
+  // that a row written and 16 rows read lie in different banks)
   u32x4 key[2][kSubs][2][NG][64];
   u32x4 value[2][kSubs][VD][VW][64];
   // ahead of the stages: their tokens' addresses, and which of them are tokens
@@ -23,8 +25,9 @@ struct TilesLds {
 };
 
 // A stage's rows on their way through registers to LDS: K as it lies, and V turned, so that a lane's
-// operand is eight tokens' of one element. A thread has one token's K row (of 64 tokens a quarter of
-// it, else an eighth) and, of eight tokens, half a chunk of V.
+// operand is eight tokens' of one element. A wave has 16 tokens' K rows (of a stage of 32 tokens half
+// of each), read row by row: read as operands, 16 bytes of 16 rows side by side, the chunks took the
+// memory pipeline four times as long. A thread has, of eight tokens, half a chunk of V.
 template <typename T, int NG, bool kWhole>
 struct Staged {
   typedef TilesLds<NG> Lds;
@@ -35,19 +38,22 @@ struct Staged {
   u32x4 k[kKeys];
   uint32_t v[8][2];
 
-  // K: wave w has rows 16 (w % (2 kSubs)) on; of 32 tokens two waves share a row, half each.
+  // The row (of 16) and chunk that the lane's n-th load of K is of.
+  static __device__ __forceinline__ void place(int n, int wave, int lane, int& row, int& chunk) {
+    const int at = 64 * (kSubs == 2 ? n : kKeys * (wave / 2) + n) + lane;
+    row = at / (4 * NG);
+    chunk = at % (4 * NG);
+  }
+
   // V: wave w has chunk column set (sub, v) = w / 2 and half w % 2.
   __device__ __forceinline__ void fetch(const FullArgs& a, const uint64_t* at, int wave, int lane) {
     const int col = lane & 15, quad = lane >> 4;
     const int rows16 = wave % (2 * kSubs);
-    const uint64_t p = at[16 * rows16 + col];
 #pragma unroll
     for (int n = 0; n < kKeys; n++) {
-      const int i = kSubs == 2 ? n : 2 * n + wave / 2;
-      if (kWhole)
-        k[n] = load16(p + 16 * quad + 64 * i);
-      else
-        k[n] = load16(p + 16 * min(4 * i + quad, a.d / 8 - 1));
+      int row, chunk;
+      place(n, wave, lane, row, chunk);
+      k[n] = load16(at[16 * rows16 + row] + 16 * (kWhole ? chunk : min(chunk, a.d / 8 - 1)));
     }
     const int sub = kSubs == 2 ? wave >> 1 : 0, vd = kSubs == 2 ? 0 : wave >> 1;
     const int e = min(VW * col + 128 * vd, a.d - VW) + VW / 2 * (wave & 1);
@@ -71,11 +77,13 @@ struct Staged {
     const int rows16 = wave % (2 * kSubs);
 #pragma unroll
     for (int n = 0; n < kKeys; n++) {
-      const int i = kSubs == 2 ? n : 2 * n + wave / 2;
+      int row, chunk;
+      place(n, wave, lane, row, chunk);
       u32x4 x = k[n];
       // elements past the head size, which the query's zeros would meet, are to be numbers
-      if (!kWhole && 8 * (4 * i + quad) >= a.d) x = u32x4{0, 0, 0, 0};
-      lds.key[stage & 1][rows16 >> 1][rows16 & 1][i][lane] = x;
+      if (!kWhole && 8 * chunk >= a.d) x = u32x4{0, 0, 0, 0};
+      lds.key[stage & 1][rows16 >> 1][rows16 & 1][chunk >> 2]
+             [16 * (chunk & 3) + (row ^ (chunk & 15))] = x;
     }
     const int sub = kSubs == 2 ? wave >> 1 : 0, vd = kSubs == 2 ? 0 : wave >> 1;
     const uint32_t ok = __builtin_amdgcn_readfirstlane(lds.ok[stage & 3][sub]);
@@ -287,7 +295,7 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
         for (int c = 0; c < NG; c++)
 #pragma unroll
           for (int g = 0; g < 2; g++) {
-            const u32x4 k = lds.key[i & 1][sub][g][c][lane];
+            const u32x4 k = lds.key[i & 1][sub][g][c][lane ^ ((4 * c + quad) & 15)];
 #pragma unroll
             for (int n = 0; n < kTiles; n++) acc[sub][g][n] = mma<T>(k, q[n][c], acc[sub][g][n]);
           }

@@ -72,54 +72,60 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       for (int r = 0; r < 4; r++) sum[g][r] = 0;
     const int from = max(t - past, 0) * static_cast<int>(a.shared.d);  // the first row that sees t
     const int row_first = from / kRowTile * kRowTile + (by_rows ? kRowTile * wave : 0);
-    u32x4 q[NG];
-    float top;
-    int sees;
-    const auto load = [&](int row0, u32x4 (&to)[NG], float& reference, int& last) {
+    // the next tiles' queries are on their way
+    struct Tile {
+      u32x4 q[NG];
+      float top;
+      int sees;  // the token of this lane's first that its row sees last
+    };
+    const auto load = [&](int row0, Tile& to) {
       uint32_t qi, qg;
       a.shared.divmod(min(row0 + col, sq.rows - 1), qi, qg);
       const int64_t token = sq.q0 + qi;
       const int q_head = head * a.shared.d + qg;
-      load_query<NG>(a, a.q + token * a.q_token + q_head * a.q_head, quad, to);
-      reference = row0 + col < sq.rows ? a.top[token * a.q_heads + q_head] : INFINITY;
-      last = past + static_cast<int>(qi) - t - 4 * quad;
+      load_query<NG>(a, a.q + token * a.q_token + q_head * a.q_head, quad, to.q);
+      to.top = row0 + col < sq.rows ? a.top[token * a.q_heads + q_head] : INFINITY;
+      to.sees = past + static_cast<int>(qi) - t - 4 * quad;
     };
-    if (row_first < sq.rows) load(row_first, q, top, sees);
-    for (int row0 = row_first; row0 < sq.rows; row0 += row_step) {
-      // the next rows are on their way
-      u32x4 q_next[NG];
-      float top_next;
-      int sees_next;
-      load(row0 + row_step, q_next, top_next, sees_next);
-      f32x4 acc[kG];
+    constexpr int kTilesAhead = 2;
+    Tile tiles[kTilesAhead];
 #pragma unroll
-      for (int g = 0; g < kG; g++) acc[g] = f32x4{0, 0, 0, 0};
+    for (int n = 0; n < kTilesAhead; n++) load(row_first + n * row_step, tiles[n]);
+    for (int row0 = row_first; row0 < sq.rows; row0 += kTilesAhead * row_step) {
 #pragma unroll
-      for (int i = 0; i < NG; i++)
+      for (int n = 0; n < kTilesAhead; n++) {
+        if (row0 + n * row_step >= sq.rows) break;
+        Tile& x = tiles[n];
+        f32x4 acc[kG];
 #pragma unroll
-        for (int g = 0; g < kG; g++) acc[g] = mma<T>(k[g][i], q[i], acc[g]);
-      // (rows that see nothing have no weights, whatever their scores)
-      const bool all = sees + 4 * quad >= kKept<NG> - 1 && top != INFINITY;
-      if (__builtin_amdgcn_ballot_w64(!all) == 0) {
+        for (int g = 0; g < kG; g++) acc[g] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int g = 0; g < kG; g++)
+        for (int i = 0; i < NG; i++)
 #pragma unroll
-          for (int r = 0; r < 4; r++)
-            sum[g][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
-      } else {
+          for (int g = 0; g < kG; g++) acc[g] = mma<T>(k[g][i], x.q[i], acc[g]);
+        const float top = x.top;
+        const int sees = x.sees;
+        load(row0 + (n + kTilesAhead) * row_step, x);
+        // (rows that see nothing have no weights, whatever their scores)
+        const bool all = sees + 4 * quad >= kKept<NG> - 1 && top != INFINITY;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!all) != 0, false)) {
+          asm volatile("");  // a branch: most rows see all of the tokens
 #pragma unroll
-        for (int g = 0; g < kG; g++)
+          for (int g = 0; g < kG; g++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float w =
-                __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
-            sum[g][r] += sees >= 16 * g + r && top != INFINITY ? w : 0.0f;
-          }
+            for (int r = 0; r < 4; r++) {
+              const float w =
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
+              sum[g][r] += sees >= 16 * g + r && top != INFINITY ? w : 0.0f;
+            }
+        } else {
+#pragma unroll
+          for (int g = 0; g < kG; g++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              sum[g][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[g][r], a.scale_log2, -top));
+        }
       }
-#pragma unroll
-      for (int i = 0; i < NG; i++) q[i] = q_next[i];
-      top = top_next;
-      sees = sees_next;
     }
     // over the rows of a tile, which are the lanes of a quarter
 #pragma unroll
