@@ -24,6 +24,8 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
                                                            FastDiv prefix_steps, FastDiv own_steps) {
   constexpr int kG = kKept<NG> / 16;
   __shared__ float s_sum[kFullWaves][kKept<NG>];
+  // a wave's queries, as full_tiles.hpp keeps keys
+  __shared__ u32x4 s_query[kFullWaves][NG][64];
   const bool prefix = blockIdx.x < prefix_items;
   const Contexts& c = prefix ? a.pre : a.own;
   const FastDiv& steps = prefix ? prefix_steps : own_steps;
@@ -72,9 +74,10 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       for (int r = 0; r < 4; r++) sum[g][r] = 0;
     const int from = max(t - past, 0) * static_cast<int>(a.shared.d);  // the first row that sees t
     const int row_first = from / kRowTile * kRowTile + (by_rows ? kRowTile * wave : 0);
-    // the next tiles' queries are on their way
+    // The next tiles' queries are on their way, read row by row (as operands, 16 bytes of 16 rows side
+    // by side, they took the memory pipeline four times as long).
     struct Tile {
-      u32x4 q[NG];
+      u32x4 x[NG];
       float top;
       int sees;  // the token of this lane's first that its row sees last
     };
@@ -83,7 +86,17 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       a.shared.divmod(min(row0 + col, sq.rows - 1), qi, qg);
       const int64_t token = sq.q0 + qi;
       const int q_head = head * a.shared.d + qg;
-      load_query<NG>(a, a.q + token * a.q_token + q_head * a.q_head, quad, to.q);
+      const uint64_t p = reinterpret_cast<uint64_t>(a.q) + token * a.q_token + q_head * a.q_head;
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+        const int row = (64 * n + lane) / (4 * NG), chunk = (64 * n + lane) % (4 * NG);
+        const uint32_t lo = __shfl(static_cast<uint32_t>(p), row);
+        const uint32_t hi = __shfl(static_cast<uint32_t>(p >> 32), row);
+        const bool in = 8 * chunk < a.d;
+        const u32x4 x = load16((static_cast<uint64_t>(hi) << 32 | lo) + (in ? 16 * chunk : 0));
+#pragma unroll
+        for (int j = 0; j < 4; j++) to.x[n][j] = in ? x[j] : 0;
+      }
       to.top = row0 + col < sq.rows ? a.top[token * a.q_heads + q_head] : INFINITY;
       to.sees = past + static_cast<int>(qi) - t - 4 * quad;
     };
@@ -96,13 +109,23 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       for (int n = 0; n < kTilesAhead; n++) {
         if (row0 + n * row_step >= sq.rows) break;
         Tile& x = tiles[n];
+        __builtin_amdgcn_wave_barrier();  // the tile before has been read
+#pragma unroll
+        for (int i = 0; i < NG; i++) {
+          const int row = (64 * i + lane) / (4 * NG), chunk = (64 * i + lane) % (4 * NG);
+          s_query[wave][chunk >> 2][16 * (chunk & 3) + (row ^ (chunk & 15))] = x.x[i];
+        }
+        __builtin_amdgcn_wave_barrier();
+        u32x4 q[NG];
+#pragma unroll
+        for (int i = 0; i < NG; i++) q[i] = s_query[wave][i][lane ^ ((4 * i + quad) & 15)];
         f32x4 acc[kG];
 #pragma unroll
         for (int g = 0; g < kG; g++) acc[g] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NG; i++)
 #pragma unroll
-          for (int g = 0; g < kG; g++) acc[g] = mma<T>(k[g][i], x.q[i], acc[g]);
+          for (int g = 0; g < kG; g++) acc[g] = mma<T>(k[g][i], q[i], acc[g]);
         const float top = x.top;
         const int sees = x.sees;
         load(row0 + (n + kTilesAhead) * row_step, x);
