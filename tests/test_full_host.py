@@ -179,16 +179,17 @@ def test_the_workspace_is_what_its_counts_need(lib):
         return got.value if rc == 0 else message(lib, rc)
 
     assert need(max_len=16) == 0  # one part a row: it is written where it goes
-    assert need(max_len=16, mass=1) == 4 * 8 * 4
+    # a reference, the running maximum and sum, and 16 scores for each of 4 x 8 rows
+    assert need(max_len=16, mass=1) == 4 * 8 * (4 + 8 + 16 * 4)
     assert need(max_len=16, groups=1, max_prefix=16) == 2 * 4 * 8 * (64 + 2) * 4
     assert need(max_len=100000) > 0
     assert need(seqs=0, tokens=0) == 0 and need(max_q=0) == 0
     assert "bad count" in need(q_heads=7)
     assert "bad count" in need(d=60)
     assert lib.evs_attend_workspace(1, 1, 1, 1, 64, 1, 1, 0, 0, 0, None) == 1
-    # longer contexts never need parts without end
+    # longer contexts never need parts without end: 1,024 of a context, 4,096 workgroups of a kind
     assert need(max_len=(1 << 31) - 1, groups=1, max_prefix=(1 << 31) - 1) <= (
-        128 * 4 * 8 * (64 + 2) * 4)
+        (1024 + 4096 // 8) * 4 * 8 * (64 + 2) * 4)
 
 
 def test_the_eviction_call_refuses_what_it_cannot_do(lib):
@@ -213,7 +214,7 @@ def test_the_eviction_call_refuses_what_it_cannot_do(lib):
     for name in ("tables", "lens", "new", "mass", "out", "kept", "ptrs"):
         assert "null" in message(lib, evict(**{name: None})), name
     assert "layers, sequences" in message(lib, evict(layers=65535, seqs=65535))
-    assert "tiles of rows" in message(lib, evict(layers=1, heads=1, seqs=1 << 21, new_width=1 << 16,
+    assert "tiles of rows" in message(lib, evict(layers=1, heads=1, seqs=1 << 20, new_width=1 << 16,
                                                  budget=1 << 20, bs=16))
     assert evict(seqs=0, lens=None) == 0
 
