@@ -220,6 +220,7 @@ constexpr int64_t kEven = 4096, kEvenChunk = 1024;
 // A context of few rows without a prefix is one part up to here: a launch less than with parts that
 // are joined. A token over 600 (8 KV heads of 128) 12.1 us for 16.5 in three parts.
 constexpr int64_t kBrief = 1024;
+constexpr int64_t kWideGroup = 512;  // rows of small chunks, from which tiles of 128 are taken
 constexpr int64_t kMostParts = 1024;
 constexpr int64_t kMostScores = int64_t{1} << 29;  // bytes of scores that a call may keep
 
@@ -274,7 +275,11 @@ Deal deal(Counts n) {
   const bool together = n.groups > 0 && shared <= kTogether;
   r.few_groups = rows <= kRowTile;
   // tiles of 128 rows where some context has them; wide heads leave no registers for them
-  const bool wide = n.d <= 128 && (most > kTogether || (together && rows / n.groups > kTogether));
+  // (Of a group of small chunks the prefix gains by them what own tokens, in tiles of few rows, lose.
+  // us with tiles of 64 and of 128: 8 sequences of 5 queries and up to 1,024 tokens behind 4 Ki, 160
+  // rows, 41 and 55; of 16 queries, 512 rows, 49 and 59; 64 of 5 behind 8 Ki, 1,280 rows, 210 and 144.)
+  const int64_t gains = most > kRowTile ? kWideGroup : kTogether;
+  const bool wide = n.d <= 128 && (most > kTogether || (together && rows / n.groups > gains));
   r.row_tiles = wide ? 2 : 1;
   const int64_t tile = kRowTile * kFullWaves * r.row_tiles;
   const bool brief = n.groups == 0 && n.max_len <= kBrief;
@@ -290,7 +295,8 @@ Deal deal(Counts n) {
   const bool busy = static_cast<int64_t>(r.few.tiles) * r.few.splits * n.heads >= 2 * kFillTiles;
   if (together)
     r.group = r.few_groups ? cut(n.groups, n.heads, n.max_prefix, kFillRows, kRound, kEven, kEvenChunk)
-                           : cut((rows + n.groups * (tile - 1)) / tile, n.heads, n.max_prefix, busy ? kFillTiles / 2 : kFillTiles, kRound, 0, kRound);
+                           : cut((rows + n.groups * (tile - 1)) / tile, n.heads, n.max_prefix,
+                                 busy ? kFillTiles / 2 : kFillTiles, kRound, 0, kRound);
   // rows that are written where they go need no parts
   r.slots = r.group.splits + (r.many.splits > 1 || r.group.splits > 0 ? r.many.splits : 0);
   r.few_slots = r.few.splits > 1 || r.group.splits > 0 ? r.few.splits : 0;
@@ -369,7 +375,9 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   EVS_REQUIRE(max_len >= 0 && max_prefix >= 0, "%s: bad count", who);
   EVS_REQUIRE(evs::good(n), "%s: bad count (%lld query heads on %lld)", who,
               static_cast<long long>(q_heads), static_cast<long long>(heads));
-  EVS_REQUIRE(scale > 0 && scale < INFINITY, "%s: the scale must be positive and finite", who);
+  const float scale_log2 = scale * 1.4426950408889634f;  // log2(e)
+  EVS_REQUIRE(scale_log2 > 0 && scale_log2 < INFINITY,
+              "%s: the scale must be positive and finite", who);
   EVS_REQUIRE(strides != nullptr, "%s: a layout is five strides", who);
   EVS_REQUIRE(strides[4] == 1, "%s: a row's elements must be contiguous (element stride %lld)", who,
               static_cast<long long>(strides[4]));
@@ -396,6 +404,9 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   EVS_REQUIRE(tokens < most / 256 &&
                   evs::workgroups(deal, heads) < most / 256,
               "%s: too many tiles of query rows", who);
+  // (workgroups that weigh: at least one a context and head, and 2^20 more)
+  EVS_REQUIRE(mass == nullptr || (seqs + groups) * heads < most / 512,
+              "%s: too many sequences and heads to weigh", who);
   EVS_REQUIRE(deal.bytes <= workspace_bytes &&
                   (deal.bytes == 0 || (workspace != nullptr &&
                                        reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
@@ -424,7 +435,7 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
   a.q_heads = static_cast<int32_t>(q_heads);
   a.shared = evs::FastDiv(static_cast<uint32_t>(q_heads / heads));
   a.div_heads = evs::FastDiv(static_cast<uint32_t>(heads));
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.group = deal.group;
   a.few = deal.few;
   a.many = deal.many;

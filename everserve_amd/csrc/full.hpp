@@ -30,6 +30,8 @@ constexpr int kRowTile = 16;  // query rows that an MFMA tile has
 // Sequences of up to kRowTile query rows a KV head take their own tokens in full_rows.hpp, others in
 // full_tiles.hpp; those of up to kTogether take a prefix with the rest of their group, and longer
 // chunks, which fill tiles by themselves, take it ahead of their own tokens, as one context.
+// us where rows beyond 16, 64 and 256 do so, behind a prefix of 4 Ki: 8 chunks of 64 rows 53, 46 and
+// 46; 8 of 128 rows 56, 56 and 53; 8 of 256 rows 87, 87 and 84; 64 of 128 rows 209, 206 and 249.
 constexpr int kTogether = 64;
 constexpr int kFullMinDim = 16;
 constexpr int kFullMaxDim = 256;

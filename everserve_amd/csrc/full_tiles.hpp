@@ -123,6 +123,12 @@ struct Staged {
 
 // One workgroup: part `item` of the contexts of tiles of 64 * kTiles query rows and one KV head,
 // 16 * kTiles rows a wave, which all take every token of a stage.
+//
+// Bound by the matrix instructions and, beside them, each score's exponential and packing: a stage of
+// tokens is read once for all rows of the tile, into registers while the stage before is computed.
+// Four chunks of 1,024 queries at the end of 4 to 8 Ki tokens, 32 heads of 128 on 8: 425 us, 848
+// TFLOP/s (a large library product: 1,197); one prompt of 4,096 from its start 192 us, 718 TFLOP/s. Of
+// few sequences a workgroup's stages are a chain of 1.7 us each, 2.3 with two workgroups a CU.
 template <typename T, int NG, bool kWhole, int kTiles>
 __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds, uint32_t item,
                                            uint32_t prefix_items) {

@@ -12,13 +12,19 @@ namespace {
 // Tokens of a wave, whose keys stay in registers while the rows pass.
 template <int NG>
 constexpr int kKept = NG > 4 ? 32 : 64;
-constexpr int kManyRows = 64;  // rows from which a workgroup's waves share them, not the tokens
+// Rows from which a workgroup's waves share them, not the tokens: each then has a tile of them.
+constexpr int kManyRows = 64;
 
 // One workgroup: the tokens of a context and KV head from kKept times `at` on, at every so-many-th
 // place. The rows of a context with many are dealt to the waves in tiles of 16, and a token's sums
-// joined in LDS; else each wave has tokens of its own. Bound by the exponentials where rows are many
-// (for 16 rows and 64 tokens 256 cycles of them, and 256 of matrix instructions, which run beside
-// them), else by reading K.
+// joined in LDS; else each wave has tokens of its own.
+//
+// Where rows are many, K stays in registers and the queries pass through LDS, so the kernel is bound by
+// its arithmetic: 64 exponentials, multiply-adds and adds a lane beside 16 matrix instructions, for 16
+// rows of 64 tokens. Two chunks of 1,024 queries that end at up to 4,001 tokens, behind 1,000 (32 heads
+// of 128 on 8): 99 us of the call's 286, which took 310 with queries read as operands. Where rows are
+// few it is bound by reading K; of few rows' own tokens the attention's scores are read instead
+// (full.hip): a decode step of 64 sequences of 1 to 4 Ki 184 us for 243.
 template <typename T, int NG>
 __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t prefix_items,
                                                            FastDiv prefix_steps, FastDiv own_steps) {
@@ -221,7 +227,6 @@ int full_weigh(const FullArgs& a, int type, int64_t max_len, int64_t max_prefix,
   const FastDiv pre(a.pre.n > 0 ? steps_of(a, max_prefix, a.pre.n, a.tokens * shared) : 1);
   const int64_t prefix_items = static_cast<int64_t>(a.pre.n) * pre.d * a.heads;
   const int64_t items = prefix_items + static_cast<int64_t>(a.own.n) * own.d * a.heads;
-  EVS_REQUIRE(items < (int64_t{1} << 23), "evs_attend: too many sequences and heads to weigh");
   if (type == EVS_BF16)
     launch<__bf16>(a, static_cast<uint32_t>(items), static_cast<uint32_t>(prefix_items), pre, own,
                    s);

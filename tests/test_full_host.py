@@ -146,7 +146,7 @@ def test_the_attention_call_refuses_what_it_cannot_do(lib):
                 dict(max_len=-1), dict(max_prefix=-1), dict(groups=-1), dict(tokens=1 << 31),
                 dict(tokens=1 << 30)):
         assert "bad count" in message(lib, attend(**bad))
-    for scale in (0.0, -1.0, math.inf, math.nan):
+    for scale in (0.0, -1.0, math.inf, math.nan, 3e38):
         assert "scale" in message(lib, attend(scale=scale))
     assert "five strides" in message(lib, attend(st=None))
     assert "contiguous" in message(lib, attend(st=strides(2048, 128, 64, 18432, 2)))
@@ -164,6 +164,8 @@ def test_the_attention_call_refuses_what_it_cannot_do(lib):
     assert "queries must" in message(lib, attend(qs=(260, 64)))
     assert "queries must" in message(lib, attend(qs=(256, 68)))
     assert "too many" in message(lib, attend(tokens=1 << 23, seqs=1 << 23, groups=0))
+    assert "to weigh" in message(lib, attend(tokens=1 << 19, seqs=1 << 19, q_heads=8, heads=8,
+                                             groups=0, mass=FAKE))
     assert "workspace" in message(lib, attend())  # a prefix's parts are joined
     assert "workspace" in message(lib, attend(size=1 << 30))
     assert "workspace" in message(lib, attend(size=1 << 30, work=ctypes.c_void_p((1 << 20) + 8)))
@@ -206,7 +208,7 @@ def test_the_eviction_call_refuses_what_it_cannot_do(lib):
         assert "bad caches" in message(lib, evict(**bad))
     for bad in (dict(width=-1), dict(seqs=-1), dict(width=1 << 28), dict(new_width=-1)):
         assert "bad tables" in message(lib, evict(**bad))
-    for bad in (dict(budget=-1, recent=0), dict(recent=41), dict(recent=-1)):
+    for bad in (dict(budget=-1, recent=0), dict(budget=(1 << 31) - 1024), dict(recent=41), dict(recent=-1)):
         assert "newest" in message(lib, evict(**bad))
     assert "hold no" in message(lib, evict(budget=49))
     assert "contiguous" in message(lib, evict(st=strides(2048, 128, 64, 18432, 2)))
