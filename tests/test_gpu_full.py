@@ -515,3 +515,23 @@ def test_what_it_cannot_do_is_refused(ext):
             call(q, tables, lens, prefix=bad)
     with pytest.raises(RuntimeError, match="scale"):
         call(q, tables, lens, scale=-1.0)
+
+
+def test_an_output_that_is_the_queries_is_refused(ext):
+    b = Batch("kv_first", 16, 2, 2, 64, "bf16", [20, 33], [1] * 2)
+    b.q = b.q.contiguous()
+    with pytest.raises(RuntimeError, match="must not be the queries"):
+        b.attend(out=b.q)
+
+
+@pytest.mark.parametrize("queries", [5, 16])
+@pytest.mark.parametrize("seqs", [8, 30, 60])
+def test_small_chunks_behind_a_prefix_on_both_sides_of_the_wide_tiles(ext, seqs, queries):
+    lens = [(7 * s + queries) % 61 + queries for s in range(seqs)]
+    Batch("kv_first", 16, 1, 4, 64, "bf16", lens, [queries] * seqs, seed=seqs, prefixes=[300],
+          groups=[0, seqs]).check()
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025])
+def test_contexts_that_are_just_one_part_and_just_two(ext, n):
+    Batch("combined", 16, 2, 4, 64, "bf16", [n, 5, n - 700], [1] * 3, seed=n).check(max_len=n)
