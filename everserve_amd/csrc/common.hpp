@@ -76,6 +76,14 @@ struct FastDiv {
   }
 };
 
+// Between a wave's accesses to LDS that its lanes make for each other: the compiler keeps them in
+// order across this (the hardware does by itself). The barrier alone orders no memory.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 inline bool aligned16(int64_t v) { return (v & 15) == 0; }
 
 // Copy `runs` runs of `len` bytes, `spitch` apart in src and `dpitch` apart in dst, on `stream`

@@ -151,9 +151,7 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
       a.div_bs.divmod(min(t, room - 1), n, off);
       const bool ok = t < static_cast<uint32_t>(stop) && page >= 0 && page < a.num_blocks;
       lds.at[wave][p & 1][lane] = base + (ok ? page * a.sb + static_cast<int64_t>(off) * a.so : 0);
-      // other lanes of the wave read them: no read is to move ahead of this, nor into a branch
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();  // other lanes of the wave read them
       return __builtin_amdgcn_ballot_w64(ok);
     };
     u32x4 q[NG];

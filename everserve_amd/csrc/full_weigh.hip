@@ -115,13 +115,13 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       for (int n = 0; n < kTilesAhead; n++) {
         if (row0 + n * row_step >= sq.rows) break;
         Tile& x = tiles[n];
-        __builtin_amdgcn_wave_barrier();  // the tile before has been read
+        wave_sync();  // the tile before has been read
 #pragma unroll
         for (int i = 0; i < NG; i++) {
           const int row = (64 * i + lane) / (4 * NG), chunk = (64 * i + lane) % (4 * NG);
           s_query[wave][chunk >> 2][16 * (chunk & 3) + (row ^ (chunk & 15))] = x.x[i];
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         u32x4 q[NG];
 #pragma unroll
         for (int i = 0; i < NG; i++) q[i] = s_query[wave][i][lane ^ ((4 * i + quad) & 15)];
@@ -163,7 +163,11 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
       for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) sum[g][r] += __shfl_xor(sum[g][r], d);
-    if (by_rows) __syncthreads();  // the sums before have been read
+    // the sums before have been read
+    if (by_rows)
+      __syncthreads();
+    else
+      wave_sync();
     if (col == 0) {
 #pragma unroll
       for (int g = 0; g < kG; g++)
@@ -173,7 +177,7 @@ __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t 
     if (by_rows)
       __syncthreads();
     else
-      __builtin_amdgcn_wave_barrier();
+      wave_sync();
     if (lane < kKept<NG> && (!by_rows || wave == 0)) {
       const uint32_t own = static_cast<uint32_t>(t) + lane;
       if (own < static_cast<uint32_t>(sq.len)) {

@@ -116,14 +116,6 @@ __device__ __forceinline__ bool writes_out(int pass, int passes) {
   return ((passes - 1 - pass) & 1) == 0;
 }
 
-// Between a wave's accesses to LDS that its lanes make for each other: the compiler keeps them in
-// order across this (the hardware does by itself).
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Count each digit of one tile, and in pass 0 OR its ids.
 template <int R>
 __global__ __launch_bounds__(kSortThreads) void count_digits(SortArgs a, int pass) {
