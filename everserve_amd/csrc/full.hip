@@ -472,8 +472,9 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
     a.stored = static_cast<int32_t>(deal.stored);
   }
   const hipStream_t s = evs::as_stream(stream);
-  if (mass != nullptr && q_starts != nullptr && deal.group.tiles > 0) {
-    // queries of a group that no sequence names have no weights
+  if (mass != nullptr && q_starts != nullptr && groups > 0) {
+    // A prefix's tokens are weighed by all queries of its group (group_rows), whichever part took the
+    // prefix: those that no sequence names, or that are past max_q, have no weights.
     const int64_t rows = tokens * q_heads;
     evs::no_weights<<<static_cast<uint32_t>((rows + 255) / 256), evs::kFullThreads, 0, s>>>(a.top,
                                                                                           rows);
