@@ -329,6 +329,33 @@ int64_t room(int64_t given, int64_t width, int64_t block_size) {
   return given == 0 ? most : least(given, most);
 }
 
+// Whether some row of the queries, `row` bytes each, has a byte of the `size` at `out`.
+bool rows_meet(const void* q, int64_t by_token, int64_t tokens, int64_t by_head, int64_t heads,
+               int64_t row, const void* out, int64_t size) {
+  typedef __int128 Wide;
+  if (by_token < 0) {  // the last token first
+    const Wide last = static_cast<Wide>(reinterpret_cast<intptr_t>(q)) +
+                      static_cast<Wide>(by_token) * (tokens - 1);
+    q = reinterpret_cast<const void*>(static_cast<intptr_t>(last));
+    by_token = -by_token;
+  }
+  const Wide from = reinterpret_cast<intptr_t>(q), at = reinterpret_cast<intptr_t>(out);
+  const Wide span = static_cast<Wide>(by_token) * (tokens - 1) + row;
+  const Wide heads_span = static_cast<Wide>(by_head) * (heads - 1);
+  if (from + (heads_span < 0 ? heads_span : 0) >= at + size ||
+      from + (heads_span > 0 ? heads_span : 0) + span <= at)
+    return false;
+  for (int64_t h = 0; h < heads; h++) {
+    // the first of the head's rows that ends behind out's start
+    const Wide first = from + static_cast<Wide>(by_head) * h;
+    const Wide short_of = at - first - row;
+    Wide t = 0;
+    if (short_of >= 0) t = by_token > 0 ? short_of / by_token + 1 : static_cast<Wide>(tokens);
+    if (t < tokens && first + t * by_token < at + size) return true;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace evs
 
@@ -412,6 +439,9 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
                                        reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
               "%s: a workspace of %lld bytes on 16, %lld needed", who,
               static_cast<long long>(workspace_bytes), static_cast<long long>(deal.bytes));
+  EVS_REQUIRE(!evs::rows_meet(q, q_strides[0] * 2, tokens, q_strides[1] * 2, q_heads, head_dim * 2,
+                              out, tokens * q_heads * head_dim * 2),
+              "%s: out must not be the queries nor overlap them: all heads' parts read them", who);
   evs::FullArgs a{};
   a.base = static_cast<char*>(const_cast<void*>(cache));
   a.sb = strides[0] * 2;

@@ -986,8 +986,6 @@ class Kernels:
             out = new((tokens, q_heads, d), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise RuntimeError("attend: out must be contiguous and like the queries")
-        elif out.data_ptr() == q.data_ptr() and out.numel():
-            raise RuntimeError("attend: out must not be the queries, which all heads' parts read")
         lse = None
         if return_lse:
             lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)

@@ -316,8 +316,8 @@ int evs_plan_compaction(const int32_t* tables, int64_t rows, int64_t width, int6
  *           the last 1; head_dim a multiple of 8, 16 to 256; rows start on 16 bytes;
  *   q       [tokens, q_heads, head_dim] of `type`, contiguous in the last; q_strides: token and head
  *           strides in elements; rows start on 16 bytes;
- *   out     contiguous [tokens, q_heads, head_dim] of `type`, starting on 16 bytes, in memory that q
- *           has no part of;
+ *   out     contiguous [tokens, q_heads, head_dim] of `type`, starting on 16 bytes; an out that
+ *           has a byte of a query row is refused;
  *   lse     contiguous f32 [tokens, q_heads], the natural log of the sum of exp(scores), or NULL;
  *   mass    contiguous f32 [num_blocks, heads, block_size], or NULL: the weight exp(score - lse) that
  *           a slot's token gets from a row, summed over the rows that see it and the query heads that
