@@ -397,6 +397,12 @@ extern "C" int evs_attend(const void* q, const int64_t* q_strides, int type, voi
               static_cast<long long>(heads));
   EVS_REQUIRE(width >= 0 && width < most && prefix_width >= 0 && prefix_width < most,
               "%s: bad table width", who);
+  // (a context of both is numbered in 32 bits)
+  EVS_REQUIRE(prefix_width == 0 || (width + prefix_width) * block_size < most,
+              "%s: tables with room for %lld tokens of prefixes and %lld behind them: 2^31 tokens are "
+              "too many",
+              who, static_cast<long long>(prefix_width * block_size),
+              static_cast<long long>(width * block_size));
   evs::Counts n{seqs,   tokens, q_heads, heads, head_dim,
                 max_q, 0,      groups,  0,     mass != nullptr};
   EVS_REQUIRE(max_len >= 0 && max_prefix >= 0, "%s: bad count", who);

@@ -327,8 +327,9 @@ int evs_plan_compaction(const int32_t* tables, int64_t rows, int64_t width, int6
  * Scores, maxima and sums are f32; a weight is rounded to `type` before it multiplies V. A row that
  * sees nothing gives zeros, and lse -infinity. A value of V that is no finite number reaches the
  * rows that see its token and no others. A table entry outside [0, num_blocks) holds nothing: its
- * tokens are masked. Lengths are taken up to their tables' room, a sequence's queries up to max_q
- * and `tokens`. Queries that no sequence names are not written. `max_len` and `max_prefix` (0: the
+ * tokens are masked. Lengths are taken up to their tables' room (and 2^31 - 1; with prefixes, own and
+ * prefix tables with room for 2^31 tokens together are refused), a sequence's queries up to max_q and
+ * `tokens`. Queries that no sequence names are not written. `max_len` and `max_prefix` (0: the
  * tables' room) are at least the longest lengths, and only steer how the work is split.
  * `workspace` is device memory of evs_attend_workspace bytes for the same counts (max_len and
  * max_prefix as the call resolves them: the tables' room where they are 0 or above it), 16-byte

@@ -47,3 +47,23 @@ SIZE = 3 * 4 * 64 * 2  # bytes of the output
 ])
 def test_an_output_among_the_queries_is_refused(lib, out, qs):
     assert "must not be the queries" in attend(lib, out=out, qs=qs)
+
+
+@pytest.mark.parametrize("width,prefix_width,bs", [
+    (1 << 10, 1 << 10, 1 << 20), (2047, 1, 1 << 20), (2047, 2047, 1 << 20), (1, (1 << 31) - 1, 1),
+    ((1 << 31) - 1, (1 << 31) - 1, (1 << 31) - 1), (1 << 30, 1, 1 << 30)])
+@pytest.mark.parametrize("groups", [0, 1])
+def test_prefixes_and_own_tokens_that_32_bits_do_not_count_are_refused(lib, width, prefix_width, bs,
+                                                                       groups):
+    """A long chunk takes its prefix and its own tokens as one context, numbered in 32 bits; parts
+    of the tables' whole room are dealt where a caller gives no bound."""
+    for bounds in (dict(), dict(max_len=1, max_prefix=1)):
+        said = attend(lib, width=width, prefix_width=prefix_width, bs=bs, groups=groups, **bounds)
+        assert "2^31 tokens" in said
+
+
+@pytest.mark.parametrize("width,prefix_width,bs", [(1 << 10, 1023, 1 << 20), (2046, 1, 1 << 20),
+                                                   (1 << 20, 0, 1 << 12), (1 << 10, (1 << 20) - 1, 1 << 10)])
+def test_room_just_below_and_wide_tables_without_prefixes_are_not(lib, width, prefix_width, bs):
+    groups = 1 if prefix_width else 0
+    assert "workspace" in attend(lib, width=width, prefix_width=prefix_width, bs=bs, groups=groups)
