@@ -186,7 +186,8 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
         float s[1][8];
 #pragma unroll
         for (int k = 0; k < 8; k++) s[0][k] = acc[k >> 2][k & 3];
-        const bool whole = t + 32 <= all_see && there == 0xFFFFFFFFu;
+        // (t + 32 may pass 2^31)
+        const bool whole = t <= all_see - 32 && there == 0xFFFFFFFFu;
         bool wild = false;
         if (__builtin_expect(!whole, false)) {
           asm volatile("");  // a branch: most tokens need none of it
@@ -205,7 +206,7 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
                 wild |= is_wild<T>(x.v[j][v][k]);
               }
           }
-          wild = t + 32 > all_see && __builtin_amdgcn_ballot_w64(wild) != 0;
+          wild = t > all_see - 32 && __builtin_amdgcn_ballot_w64(wild) != 0;
         }
         float fade[1];
         if (grow<1>(s, a.scale_log2, run, fade)) {

@@ -270,7 +270,10 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
 #pragma unroll
     for (int k = 0; k < 3; k++) locate(k, pages[k]);
     __syncthreads();
-    const auto tame = [&](int stage) { return begin + (stage + 1) * kTokens > tile_see; };
+    const auto tame = [&](int stage) {  // (its end may pass 2^31)
+      return static_cast<uint32_t>(begin) + static_cast<uint32_t>((stage + 1) * kTokens) >
+             static_cast<uint32_t>(tile_see);
+    };
     Staged<T, NG, kWhole> rows;
     rows.fetch(a, lds.at[0], wave, lane);
     rows.store(a, lds, 0, wave, lane, tame(0));
@@ -316,7 +319,7 @@ __device__ __forceinline__ void tiles_part(const FullArgs& a, TilesLds<NG>& lds,
         ok[sub] = __builtin_amdgcn_readfirstlane(lds.ok[i & 3][sub]);
         all &= ok[sub];
       }
-      if (__builtin_expect(t0 + kTokens > all_see || all != 0xFFFFFFFFu, false)) {
+      if (__builtin_expect(t0 > all_see - kTokens || all != 0xFFFFFFFFu, false)) {
         asm volatile("");  // a branch: most stages need none of it
 #pragma unroll
         for (int sub = 0; sub < kSubs; sub++)
