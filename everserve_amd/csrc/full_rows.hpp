@@ -150,6 +150,7 @@ __device__ __forceinline__ void rows_part(const FullArgs& a, RowsLds<NG>& lds, u
       uint32_t n, off;
       a.div_bs.divmod(min(t, room - 1), n, off);
       const bool ok = t < static_cast<uint32_t>(stop) && page >= 0 && page < a.num_blocks;
+      wave_sync();  // those before have been read
       lds.at[wave][p & 1][lane] = base + (ok ? page * a.sb + static_cast<int64_t>(off) * a.so : 0);
       wave_sync();  // other lanes of the wave read them
       return __builtin_amdgcn_ballot_w64(ok);

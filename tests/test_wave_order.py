@@ -30,6 +30,25 @@ def test_a_waves_barrier_stands_behind_a_fence(path):
     assert unfenced(path.read_text()) == []
 
 
+# where a wave's lanes write what its other lanes read
+EXCHANGES = [("full_rows.hpp", "lds.at[wave]"), ("full_weigh.hip", "s_query[wave]"),
+             ("full_weigh.hip", "s_sum[wave]")]
+SYNC = re.compile(r"\b(wave_sync|__syncthreads)\(\);")
+
+
+@pytest.mark.parametrize("name,array", EXCHANGES, ids=lambda x: x.split("[")[0])
+def test_a_waves_writes_stand_between_waits_of_it(name, array):
+    """Those ahead for the reads of what was there before, those behind for the reads of them."""
+    text = code_of(next(p for p in SOURCES if p.name == name).read_text())
+    stores = [m.start() for m in re.finditer(re.escape(array) + r"[^;{}]*\]\s*=[^=]", text)]
+    assert len(stores) == 1
+    before = [m.end() for m in SYNC.finditer(text, 0, stores[0])]
+    behind = SYNC.search(text, stores[0])
+    assert before and behind
+    between = text[before[-1]:behind.start()]
+    assert between.count(array) == 1, between  # the store alone
+
+
 def test_a_barrier_without_one_is_found():
     bare = "s[lane] = x;\n  __builtin_amdgcn_wave_barrier();  // read by others\n  y = s[0];"
     assert unfenced(bare) == ["s[lane] = x"]
