@@ -218,7 +218,11 @@ constexpr int64_t kFillTiles = 256;  // and of many
 // Beyond that, workgroups for few rows of contexts of unlike lengths, and the tokens of one.
 constexpr int64_t kEven = 4096, kEvenChunk = 1024;
 // A context of few rows without a prefix is one part up to here: a launch less than with parts that
-// are joined. A token over 600 (8 KV heads of 128) 12.1 us for 16.5 in three parts.
+// are joined. us of calls in a row, and replayed from a graph, on 8 KV heads of 128, in one part (and in
+// parts of 256): one token over 600 11.5, 11.3 (12.4, 11.0), over 1,000 13.5, 13.4 (12.7, 11.4); 16
+// sequences of 600 13.4, 13.5 (17.4, 17.2), of 1,000 16.5, 16.6 (20.1, 20.1). With mass the second
+// launch follows either way and parts would be faster (one of 600 17.3 (12.9), 16 of 1,000 23.0 (20.5)),
+// but a call gives the same bits with mass and without, so both are cut alike.
 constexpr int64_t kBrief = 1024;
 constexpr int64_t kWideGroup = 512;  // rows of small chunks, from which tiles of 128 are taken
 constexpr int64_t kMostParts = 1024;

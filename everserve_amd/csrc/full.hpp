@@ -15,7 +15,10 @@
 // between them: the scores leave a lane with four tokens of one query row, and those weights are its
 // part of the second operand as they stand. A weight exp(s - m) is rounded to the cache's type before
 // it multiplies V (bf16: at most 2^-8 of it, f16: 2^-11 or, below 2^-14, 2^-25 in all); the sum of
-// the weights is taken before that.
+// the weights is taken before that. The matrix instructions take 16 bits, and a weight's rest as a
+// second term would make them half as many again, which bound chunks, for less than the output's own
+// rounding: answers are off from 64 bits by 0.0019 to 0.0023 of their norm in bf16 (f16: 0.00027),
+// f32 sums rounded once by 0.0016 to 0.0017 (0.00021).
 #pragma once
 
 #include <type_traits>

@@ -1,9 +1,12 @@
 // The weights that tokens got in an attention over full-width pages, added to their mass.
 //
 // The weight of token t for row r is exp(s_rt - lse_r), with the row's lse from the attention before
-// it; a token's mass of a KV head grows by their sum over the rows of that head that see it. Each
-// token and head has one wave, which takes the rows in order: no atomics, and the same sums in every
-// run. A prefix's tokens get the weights of all rows of its group at once.
+// it; a token's mass of a KV head grows by their sum over the rows of that head that see it. The sum
+// is formed by the wave that has the token, row tile by row tile; from 64 rows on by the four waves of
+// a workgroup, which share the rows and join their sums in LDS; or, of few rows' own tokens, by a
+// thread from the scores that the attention kept (weigh_scores in full.hip). Each in a fixed order,
+// without atomics: the same sums in every run. A prefix's tokens get the weights of all rows of its
+// group at once.
 #include "full.hpp"
 
 namespace evs {
@@ -20,8 +23,8 @@ constexpr int kManyRows = 64;
 // joined in LDS; else each wave has tokens of its own.
 //
 // Where rows are many, K stays in registers and the queries pass through LDS, so the kernel is bound by
-// its arithmetic: 64 exponentials, multiply-adds and adds a lane beside 16 matrix instructions, for 16
-// rows of 64 tokens. Two chunks of 1,024 queries that end at up to 4,001 tokens, behind 1,000 (32 heads
+// its vector arithmetic: for 16 rows of 64 tokens of 128 elements some 130 instructions, 16
+// exponentials, multiply-adds and adds among them, beside 16 matrix instructions. Two chunks of 1,024 queries that end at up to 4,001 tokens, behind 1,000 (32 heads
 // of 128 on 8): 99 us of the call's 286, which took 310 with queries read as operands. Where rows are
 // few it is bound by reading K; of few rows' own tokens the attention's scores are read instead
 // (full.hip): a decode step of 64 sequences of 1 to 4 Ki 184 us for 243.
