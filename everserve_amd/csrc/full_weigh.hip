@@ -24,10 +24,11 @@ constexpr int kManyRows = 64;
 //
 // Where rows are many, K stays in registers and the queries pass through LDS, so the kernel is bound by
 // its vector arithmetic: for 16 rows of 64 tokens of 128 elements some 130 instructions, 16
-// exponentials, multiply-adds and adds among them, beside 16 matrix instructions. Two chunks of 1,024 queries that end at up to 4,001 tokens, behind 1,000 (32 heads
-// of 128 on 8): 99 us of the call's 286, which took 310 with queries read as operands. Where rows are
-// few it is bound by reading K; of few rows' own tokens the attention's scores are read instead
-// (full.hip): a decode step of 64 sequences of 1 to 4 Ki 184 us for 243.
+// exponentials, multiply-adds and adds among them, beside 16 matrix instructions. Two chunks of 1,024
+// queries that end at up to 4,001 tokens, behind 1,000 (32 heads of 128 on 8): 99 us of the call's 288,
+// which took 310 with queries read as operands. Where rows are few it is bound by reading K; of few
+// rows' own tokens the attention's scores are read instead (full.hip): a decode step of 64 sequences
+// of 1 to 4 Ki 185 us for 243.
 template <typename T, int NG>
 __global__ __launch_bounds__(kFullThreads) void weigh_full(FullArgs a, uint32_t prefix_items,
                                                            FastDiv prefix_steps, FastDiv own_steps) {

@@ -50,8 +50,15 @@ class Evictor(PageMover):
         and those that it gets; the latter must have room for the budget, be named once, and none
         of them be in ``block_tables``. Shorter sequences move as they are. ``mass`` (f32 [layers,
         num_blocks, heads, block_size], contiguous) moves with the rows. Pages outside the cache hold
-        nothing: their tokens go first, and nothing moves from or to them. Two launches on the
-        current stream; lengths and tables are read on the device, so it may be captured."""
+        nothing: their tokens go first, and nothing moves from or to them. One of them that stays
+        all the same (one of the newest, or where there are no more than the budget) counts in the
+        new length, and its new slot holds what it held, for attention to see: evict sequences whose
+        pages are all there. Two launches on the current stream; lengths and tables are read on the
+        device, so it may be captured.
+
+        Masses of pages that are filled by other means are the caller's to set: :meth:`copy`,
+        :meth:`compact` and a restore move rows alone (``mass[:, dst] = mass[:, src]`` with a
+        copy's or a plan's pages, 0 for restored ones)."""
         return Eviction(*_kernels().evict(self._ptrs, self.num_blocks, self.num_heads,
                                           self.head_dim, self.block_size, self._strides, self.elem,
                                           block_tables, seq_lens, new_tables, budget, mass, recent))

@@ -358,7 +358,9 @@ int evs_attend(const void* q, const int64_t* q_strides, int type, void* out, flo
  * lens_out[s] (device, int32) gets the tokens that stay, kept (device, contiguous int32 [num_layers,
  * seqs, heads, budget]) which they are, -1 past them. The pages of `tables` are only read, so other
  * sequences may share them; those of new_tables must be named once and in none of `tables`. Rows and
- * mass from and to pages outside the cache are not moved. Two launches; nothing is allocated. */
+ * mass from and to pages outside the cache are not moved: a token there that stays, as one of the
+ * newest or of no more than the budget, counts in lens_out, and its new slot, which attention then
+ * sees, holds what it held. Two launches; nothing is allocated. */
 int evs_evict(const int64_t* layer_ptrs, int64_t num_layers, int64_t num_blocks, int64_t num_heads,
               int64_t head_dim, int64_t block_size, const int64_t* strides, int64_t elem_size,
               const int32_t* tables, int64_t table_stride, int64_t width, const int32_t* lens,
